@@ -12,7 +12,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libcgnn_hip.so")
 
-F32, F64 = 0, 1
+F32, F64, F16, BF16 = 0, 1, 2, 3
 SPMM_AUTO, SPMM_ROW, SPMM_NNZ = 0, 1, 2
 
 EXPORTS = [
@@ -31,6 +31,7 @@ EXPORTS = [
     "cgnn_reconstruct_backward_signs", "cgnn_reconstruct_masks", "cgnn_reconstruct_backward_masks", "cgnn_copy_bytes", "cgnn_read_bytes", "cgnn_fill_bytes",
     "cgnn_exclusive_sum_workspace_bytes", "cgnn_exclusive_sum_i32", "cgnn_sample_count", "cgnn_sample_fill",
     "cgnn_sample_relabel_begin", "cgnn_sample_relabel_workspace_bytes", "cgnn_sample_relabel", "cgnn_sample_layers_workspace_bytes", "cgnn_sample_layers", "cgnn_sample_layers_write",
+    "cgnn_dropout", "cgnn_layer_norm", "cgnn_layer_norm_backward_workspace_bytes", "cgnn_layer_norm_backward",
 ]
 
 
@@ -46,6 +47,10 @@ class CsrStruct(ctypes.Structure):
         ("wg_runs", ctypes.c_void_p), ("arrivals", ctypes.c_void_p),
         ("wg_groups", ctypes.c_int32), ("wg_len", ctypes.c_int32),
     ]
+
+
+class DropStruct(ctypes.Structure):
+    _fields_ = [("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64), ("counter", ctypes.c_void_p), ("kept", ctypes.c_int32)]
 
 
 _lib = None
@@ -64,7 +69,8 @@ def lib():
                      "cgnn_cluster_members_workspace_bytes", "cgnn_cluster_mean_workspace_bytes",
                      "cgnn_csr_transpose_workspace_bytes", "cgnn_compress_batch_workspace_bytes",
                      "cgnn_sample_layers_workspace_bytes", "cgnn_spmm_once_workspace_bytes", "cgnn_cluster_sums_workspace_bytes", "cgnn_column_sums_workspace_bytes",
-                     "cgnn_exclusive_sum_workspace_bytes", "cgnn_sample_relabel_workspace_bytes"):
+                     "cgnn_exclusive_sum_workspace_bytes", "cgnn_sample_relabel_workspace_bytes",
+                     "cgnn_layer_norm_backward_workspace_bytes"):
             getattr(L, name).restype = ctypes.c_size_t
         L.cgnn_lsh_group_small_rows.restype = ctypes.c_int64
         _lib = L
@@ -376,3 +382,49 @@ def reconstruct_backward(grad, output, members, groups, relu=False, max_members=
                                       ctypes.c_int(1 if relu else 0), ptr(reps_grad), ptr(ws),
                                       ctypes.c_size_t(need), stream_of(grad)))
     return reps_grad
+
+
+ROW_DTYPES = {torch.float32: F32, torch.float64: F64, torch.float16: F16, torch.bfloat16: BF16}
+
+
+def drop_struct(p, seed, offset=0, counter=None):
+    """The mask that keeps a share of 1 - p, to the nearest 65,536th."""
+    low = (1 << 64) - 1
+    return DropStruct(seed & low, offset & low, 0 if counter is None else counter.data_ptr(), int((1 - p) * 65536 + 0.5))
+
+
+def dropout(x, p, seed, offset=0, counter=None):
+    """x: [rows, F], its rows any number of elements apart."""
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    check(lib().cgnn_dropout(i64(x.shape[0]), i64(x.shape[1]), ROW_DTYPES[x.dtype], ptr(x), i64(x.stride(0)),
+                             ctypes.byref(drop_struct(p, seed, offset, counter)), ptr(out), stream_of(x)))
+    return out
+
+
+def _param_dtype(x, weight, bias):
+    return next((ROW_DTYPES[t.dtype] for t in (weight, bias) if t is not None), ROW_DTYPES[x.dtype])
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, relu=False, drop=None):
+    """(out, stats) through cgnn_layer_norm; drop: a DropStruct or None."""
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty((x.shape[0], 2), dtype=torch.float64, device=x.device)
+    check(lib().cgnn_layer_norm(i64(x.shape[0]), i64(x.shape[1]), ROW_DTYPES[x.dtype], _param_dtype(x, weight, bias), ptr(x),
+                                i64(x.stride(0)), ptr(weight), ptr(bias), ctypes.c_double(eps), ctypes.c_int(1 if relu else 0),
+                                None if drop is None else ctypes.byref(drop), ptr(out), ptr(stats), stream_of(x)))
+    return out, stats
+
+
+def layer_norm_backward(grad, x, stats, weight=None, bias=None, relu=False, drop=None):
+    """(dx, dweight, dbias) through cgnn_layer_norm_backward."""
+    rows, F = x.shape
+    kind = next((t.dtype for t in (weight, bias) if t is not None), x.dtype)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dweight, dbias = (torch.empty(F, dtype=kind, device=x.device) for _ in range(2))
+    need = lib().cgnn_layer_norm_backward_workspace_bytes(i64(rows), i64(F), ROW_DTYPES[x.dtype])
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=x.device)
+    check(lib().cgnn_layer_norm_backward(
+        i64(rows), i64(F), ROW_DTYPES[x.dtype], _param_dtype(x, weight, bias), ptr(grad), i64(grad.stride(0)), ptr(x), i64(x.stride(0)),
+        ptr(stats), ptr(weight), ptr(bias), ctypes.c_int(1 if relu else 0), None if drop is None else ctypes.byref(drop), ptr(dx),
+        ptr(dweight), ptr(dbias), ptr(ws), ctypes.c_size_t(need), stream_of(x)))
+    return dx, dweight, dbias

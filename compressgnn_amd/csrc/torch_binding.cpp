@@ -1637,6 +1637,261 @@ c10::optional<Tensor> reconstruct(Tensor reps, Tensor index, c10::optional<Tenso
     return rows;
 }
 
+// ------------------------------------------- between two layers: norm and dropout ----
+
+// A tensor as rows of its last dimension: dense ones and matrices whose rows lie apart as they are, others as a dense copy.
+struct Rows {
+    Tensor data;
+    int64_t count, width, stride;
+};
+
+Rows rows_of(const char *op, const char *name, const Tensor &t) {
+    const auto type = t.defined() ? t.scalar_type() : torch::kBool;
+    TORCH_CHECK(t.defined() && t.is_cuda() && t.layout() == torch::kStrided &&
+                    (type == torch::kFloat32 || type == torch::kFloat64 || type == torch::kFloat16 || type == torch::kBFloat16),
+                op, ": ", name, " has to be a float32, float64, float16 or bfloat16 tensor on the GPU; it is ",
+                !t.defined() ? "undefined" : t.layout() == torch::kStrided ? seen(t) : c10::str(type, t.sizes(), " of layout ", t.layout()));
+    const int64_t width = t.dim() ? t.size(-1) : 1;
+    const Tensor plain = t.is_neg() ? t.resolve_neg() : t;
+    if (plain.dim() == 2 && (width <= 1 || plain.stride(1) == 1)) return {plain, plain.size(0), width, plain.stride(0)};
+    const Tensor dense = plain.contiguous();
+    return {dense, width ? dense.numel() / width : 0, width, width};
+}
+
+int row_dtype(const Tensor &t) {
+    switch (t.scalar_type()) {
+        case torch::kFloat32: return CGNN_F32;
+        case torch::kFloat64: return CGNN_F64;
+        case torch::kFloat16: return CGNN_F16;
+        default: return CGNN_BF16;
+    }
+}
+
+// The mask of a call: p, seed, offset and, where the program keeps one, the device counter that is added to it.
+struct Masked {
+    double p = 0;
+    int64_t seed = 0, offset = 0;
+    Tensor counter;
+    bool drops() const { return kept() < 65536; }
+    int32_t kept() const { return (int32_t)std::floor((1.0 - p) * 65536.0 + 0.5); }
+    cgnn_drop view() const {
+        return {(uint64_t)seed, (uint64_t)offset, counter.defined() ? counter.data_ptr<int64_t>() : nullptr, kept()};
+    }
+};
+
+Masked masked_by(const char *op, const Tensor &x, double p, int64_t seed, int64_t offset, const c10::optional<Tensor> &counter) {
+    TORCH_CHECK(p >= 0 && p <= 1, op, ": p has to lie in [0, 1]; it is ", p);
+    Masked m{p, seed, offset, counter.has_value() ? *counter : Tensor()};
+    TORCH_CHECK(!m.counter.defined() || (m.counter.device() == x.device() && m.counter.scalar_type() == torch::kInt64 &&
+                                         m.counter.layout() == torch::kStrided && m.counter.numel() == 1),
+                op, ": counter has to be an int64 tensor of one element beside x; it is ", m.counter.defined() ? seen(m.counter) : "");
+    return m;
+}
+
+Tensor dropout_rows(const char *op, const char *name, const Tensor &x, const Masked &m) {
+    const Rows rows = rows_of(op, name, x);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    Tensor out = torch::empty(x.sizes(), x.options().memory_format(torch::MemoryFormat::Contiguous));
+    if (out.numel() == 0) return out;
+    const cgnn_drop drop = m.view();
+    ok(cgnn_dropout(rows.count, rows.width, row_dtype(x), rows.data.data_ptr(), rows.stride, &drop, out.data_ptr(), current_stream(x)), op);
+    return out;
+}
+
+// One application without autograd: the forward pass, or the gradient where x is the output's.
+Tensor dropout_forward(Tensor x, double p, int64_t seed, int64_t offset, c10::optional<Tensor> counter) {
+    return dropout_rows("dropout", "x", x, masked_by("dropout", x, p, seed, offset, counter));
+}
+
+struct DropoutBackward : torch::autograd::Node {
+    Masked mask;
+    torch::autograd::SavedVariable counter;
+    torch::autograd::variable_list apply(torch::autograd::variable_list &&grads) override {
+        if (!grads[0].defined()) return {Tensor()};
+        const bool recorded = at::GradMode::is_enabled();
+        Tensor out;
+        {
+            at::NoGradGuard no_grad;
+            Masked m = mask;
+            m.counter = counter.unpack();
+            out = dropout_rows("dropout backward", "grad", grads[0], m);
+        }
+        return first_order({out}, recorded);
+    }
+    void release_variables() override { counter.reset_data(); }
+    std::string name() const override { return "DropoutBackward"; }
+};
+
+c10::optional<Tensor> dropout(Tensor x, double p, int64_t seed, int64_t offset, c10::optional<Tensor> counter) {
+    if (needs_function(x)) return c10::nullopt;
+    Masked m = masked_by("dropout", x, p, seed, offset, counter);
+    Tensor out;
+    {
+        at::AutoDispatchBelowADInplaceOrView plain;
+        out = dropout_rows("dropout", "x", x, m);
+    }
+    if (at::GradMode::is_enabled() && x.requires_grad()) {
+        auto node = node_over<DropoutBackward>(x);
+        node->counter = torch::autograd::SavedVariable(m.counter, false);
+        m.counter = Tensor();
+        node->mask = std::move(m);
+        torch::autograd::set_history(out, node);
+    }
+    return out;
+}
+
+// weight and bias as the kernels take them: dense, and of one type.
+struct NormParams {
+    Tensor weight, bias;
+    int dtype = 0;
+    const void *of(const Tensor &t) const { return t.defined() ? t.data_ptr() : nullptr; }
+};
+
+NormParams norm_params(const char *op, const Tensor &x, const c10::optional<Tensor> &weight, const c10::optional<Tensor> &bias) {
+    NormParams p;
+    p.dtype = row_dtype(x);
+    auto take = [&](const c10::optional<Tensor> &given, const char *name) {
+        if (!given.has_value() || !given->defined()) return Tensor();
+        const Tensor &t = *given;
+        const bool wide = t.scalar_type() == torch::kFloat32 && x.scalar_type() != torch::kFloat64;
+        TORCH_CHECK(t.device() == x.device() && t.layout() == torch::kStrided && t.dim() == 1 && t.size(0) == x.size(-1) &&
+                        (t.scalar_type() == x.scalar_type() || wide),
+                    op, ": ", name, " has to be a vector of ", x.size(-1), " entries beside x, of its type or float32 beside 16-bit rows; it is ",
+                    seen(t));
+        p.dtype = wide ? CGNN_F32 : row_dtype(t);
+        return (t.is_neg() ? t.resolve_neg() : t).contiguous();
+    };
+    p.weight = take(weight, "weight");
+    p.bias = take(bias, "bias");
+    TORCH_CHECK(!p.weight.defined() || !p.bias.defined() || p.weight.scalar_type() == p.bias.scalar_type(), op,
+                ": weight and bias have to be of one type; they are ", p.weight.scalar_type(), " and ", p.bias.scalar_type());
+    return p;
+}
+
+// (out, statistics or undefined)
+std::tuple<Tensor, Tensor> norm_rows(const char *op, const Rows &rows, const Tensor &x, const NormParams &params, double eps, bool relu,
+                                     const Masked &m, bool with_stats) {
+    TORCH_CHECK(eps >= 0 && std::isfinite(eps), op, ": eps has to be a finite number of at least 0; it is ", eps);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    Tensor out = torch::empty(x.sizes(), x.options().memory_format(torch::MemoryFormat::Contiguous)), stats;
+    if (with_stats) stats = torch::empty({rows.count, 2}, x.options().dtype(torch::kFloat64));
+    if (out.numel() == 0) return {out, stats};
+    const cgnn_drop drop = m.view();
+    ok(cgnn_layer_norm(rows.count, rows.width, row_dtype(x), params.dtype, rows.data.data_ptr(), rows.stride, params.of(params.weight),
+                       params.of(params.bias), eps, relu, m.drops() ? &drop : nullptr, out.data_ptr(),
+                       with_stats ? stats.data_ptr<double>() : nullptr, current_stream(x)),
+       op);
+    return {out, stats};
+}
+
+// {dx, dweight, dbias}, those that `wanted` asks for.
+std::array<Tensor, 3> norm_gradients(const char *op, const Tensor &grad, const Tensor &x, const Tensor &stats, const NormParams &params,
+                                     bool relu, const Masked &m, std::array<bool, 3> wanted) {
+    const Rows rows = rows_of(op, "x", x), d = rows_of(op, "grad", grad);
+    TORCH_CHECK(grad.sizes() == x.sizes() && grad.scalar_type() == x.scalar_type() && grad.device() == x.device(), op,
+                ": grad has to be of the size and type of x and beside it; x is ", seen(x), ", grad ", seen(grad));
+    TORCH_CHECK(stats.device() == x.device() && stats.scalar_type() == torch::kFloat64 && stats.is_contiguous() && stats.dim() == 2 &&
+                    stats.size(0) == rows.count && stats.size(1) == 2,
+                op, ": the statistics have to be a contiguous float64 tensor [", rows.count, ", 2] beside x; they are ", seen(stats));
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    std::array<Tensor, 3> out;
+    if (wanted[0]) out[0] = torch::empty(x.sizes(), x.options().memory_format(torch::MemoryFormat::Contiguous));
+    const auto kind = x.options().dtype(params.weight.defined() ? params.weight.scalar_type()
+                                        : params.bias.defined() ? params.bias.scalar_type() : x.scalar_type());
+    for (int i : {1, 2})
+        if (wanted[i]) out[i] = x.numel() ? torch::empty({rows.width}, kind) : torch::zeros({rows.width}, kind);
+    if (x.numel() == 0) return out;
+    const size_t bytes = wanted[1] || wanted[2] ? cgnn_layer_norm_backward_workspace_bytes(rows.count, rows.width, row_dtype(x)) : 0;
+    Tensor workspace;
+    if (bytes) workspace = torch::empty({(int64_t)bytes}, x.options().dtype(torch::kUInt8));
+    const cgnn_drop drop = m.view();
+    ok(cgnn_layer_norm_backward(rows.count, rows.width, row_dtype(x), params.dtype, d.data.data_ptr(), d.stride, rows.data.data_ptr(),
+                                rows.stride, stats.data_ptr<double>(), params.of(params.weight), params.of(params.bias), relu,
+                                m.drops() ? &drop : nullptr, out[0].defined() ? out[0].data_ptr() : nullptr,
+                                out[1].defined() ? out[1].data_ptr() : nullptr, out[2].defined() ? out[2].data_ptr() : nullptr,
+                                bytes ? workspace.data_ptr() : nullptr, bytes, current_stream(x)),
+       op);
+    return out;
+}
+
+std::tuple<Tensor, Tensor> layer_norm_forward(Tensor x, c10::optional<Tensor> weight, c10::optional<Tensor> bias, double eps, bool relu,
+                                              double p, int64_t seed, int64_t offset, c10::optional<Tensor> counter) {
+    const char *op = "layer_norm";
+    const Rows rows = rows_of(op, "x", x);
+    TORCH_CHECK(x.dim() >= 1, op, ": x has no last dimension to normalise over");
+    return norm_rows(op, rows, x, norm_params(op, x, weight, bias), eps, relu, masked_by(op, x, p, seed, offset, counter), true);
+}
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(Tensor grad, Tensor x, Tensor stats, c10::optional<Tensor> weight,
+                                                       c10::optional<Tensor> bias, bool relu, double p, int64_t seed, int64_t offset,
+                                                       c10::optional<Tensor> counter) {
+    const char *op = "layer_norm_backward";
+    rows_of(op, "x", x);
+    TORCH_CHECK(x.dim() >= 1, op, ": x has no last dimension");
+    auto out = norm_gradients(op, grad, x, stats, norm_params(op, x, weight, bias), relu, masked_by(op, x, p, seed, offset, counter),
+                              {true, true, true});
+    return {out[0], out[1], out[2]};
+}
+
+struct NormBackward : torch::autograd::Node {
+    torch::autograd::SavedVariable x, stats, weight, bias, counter;
+    Masked mask;
+    bool relu = false;
+    torch::autograd::variable_list apply(torch::autograd::variable_list &&grads) override {
+        if (!grads[0].defined()) return torch::autograd::variable_list(3);
+        const bool recorded = at::GradMode::is_enabled();
+        torch::autograd::variable_list out;
+        {
+            at::NoGradGuard no_grad;
+            Masked m = mask;
+            m.counter = counter.unpack();
+            const Tensor rows = x.unpack();
+            const NormParams params = norm_params("layer_norm backward", rows, weight.unpack(), bias.unpack());
+            std::array<bool, 3> wanted;
+            for (size_t i = 0; i < 3; ++i) wanted[i] = task_should_compute_output(i);
+            for (Tensor &g : norm_gradients("layer_norm backward", grads[0], rows, stats.unpack(), params, relu, m, wanted))
+                out.push_back(std::move(g));
+        }
+        return first_order(std::move(out), recorded);
+    }
+    void release_variables() override {
+        for (auto *saved : {&x, &stats, &weight, &bias, &counter}) saved->reset_data();
+    }
+    std::string name() const override { return "LayerNormBackward"; }
+};
+
+// drop(relu(layer_norm(x))) with its gradients.  Kept for them: x, its parameters, and mean and deviation of every row; neither
+// the normalised rows nor a mask.
+c10::optional<Tensor> layer_norm(Tensor x, c10::optional<Tensor> weight, c10::optional<Tensor> bias, double eps, bool relu, double p,
+                                 int64_t seed, int64_t offset, c10::optional<Tensor> counter) {
+    const char *op = "layer_norm";
+    const Tensor w = weight.has_value() ? *weight : Tensor(), b = bias.has_value() ? *bias : Tensor();
+    if (needs_function(x, weight) || (b.defined() && b._fw_grad(0).defined())) return c10::nullopt;
+    const Rows rows = rows_of(op, "x", x);
+    TORCH_CHECK(x.dim() >= 1, op, ": x has no last dimension to normalise over");
+    Masked m = masked_by(op, x, p, seed, offset, counter);
+    const bool recorded = at::GradMode::is_enabled() && (x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad()));
+    Tensor out, stats;
+    {
+        at::AutoDispatchBelowADInplaceOrView plain;
+        std::tie(out, stats) = norm_rows(op, rows, x, norm_params(op, x, weight, bias), eps, relu, m, recorded);
+    }
+    if (recorded) {
+        std::shared_ptr<NormBackward> node(new NormBackward(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(x, w, b));
+        node->x = torch::autograd::SavedVariable(x, false);
+        node->stats = torch::autograd::SavedVariable(stats, false);
+        node->weight = torch::autograd::SavedVariable(w, false);
+        node->bias = torch::autograd::SavedVariable(b, false);
+        node->counter = torch::autograd::SavedVariable(m.counter, false);
+        m.counter = Tensor();
+        node->mask = std::move(m);
+        node->relu = relu;
+        torch::autograd::set_history(out, node);
+    }
+    return out;
+}
+
 // (colptr, row, value) of a block held as int64 tensors on a GPU: the CSR of its transpose,
 // in the order SparseTensor.csc() gives.  The one host read (a flag for columns out of
 // range) comes after the last kernel.
@@ -2115,6 +2370,19 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("reconstruct", &reconstruct, "act(reps[index] + bias) with its gradients", py::arg("reps"), py::arg("index"),
           py::arg("bias"), py::arg("relu"), py::arg("members") = py::none());
     m.def("column_sums", &column_sums, "sum over the rows of a matrix");
+    m.def("dropout", &dropout, "elements dropped by position, with the gradient", py::arg("x"), py::arg("p"), py::arg("seed"),
+          py::arg("offset") = 0, py::arg("counter") = py::none());
+    m.def("layer_norm", &layer_norm, "layer norm, ReLU and dropout of rows in one pass, with the gradients", py::arg("x"),
+          py::arg("weight") = py::none(), py::arg("bias") = py::none(), py::arg("eps") = 1e-5, py::arg("relu") = false, py::arg("p") = 0.0,
+          py::arg("seed") = 0, py::arg("offset") = 0, py::arg("counter") = py::none());
+    m.def("dropout_forward", &dropout_forward, "dropout without autograd; its own gradient", py::arg("x"), py::arg("p"), py::arg("seed"),
+          py::arg("offset") = 0, py::arg("counter") = py::none());
+    m.def("layer_norm_forward", &layer_norm_forward, "(rows, [mean, 1 / deviation] of every row), without autograd", py::arg("x"),
+          py::arg("weight"), py::arg("bias"), py::arg("eps"), py::arg("relu") = false, py::arg("p") = 0.0, py::arg("seed") = 0,
+          py::arg("offset") = 0, py::arg("counter") = py::none());
+    m.def("layer_norm_backward", &layer_norm_backward, "gradients of x, weight and bias", py::arg("grad"), py::arg("x"), py::arg("stats"),
+          py::arg("weight"), py::arg("bias"), py::arg("relu") = false, py::arg("p") = 0.0, py::arg("seed") = 0, py::arg("offset") = 0,
+          py::arg("counter") = py::none());
     m.def("propagate", &propagate, "plan.forward(x) with plan.backward as its gradient", py::arg("plan"), py::arg("x"),
           py::arg("once_differentiable") = false);
     m.def("version", []() { return std::string(cgnn_version()); });

@@ -1,0 +1,90 @@
+"""Dropout of node features whose mask is never stored: out = x / (1 - p) where an element is kept, else 0.
+
+The reference's models take dropout from torch; here it is a kernel that finds the mask from (seed, offset) and the
+position of an element, in the forward pass and again in the gradient.  The share of kept elements is taken to the
+nearest 65,536th and the scale is its reciprocal.  Rows are the last dimension; the mask of an element depends on its row and
+its column, not on the type or on strides.
+"""
+import _paths  # noqa: F401
+import torch
+from torch.autograd.function import once_differentiable
+
+import compressgnn_runtime as _native
+
+
+class _Dropped(torch.autograd.Function):
+    """(x, p, seed, offset, counter) -> out: the step of _native.dropout, for what a native one does not take part in"""
+
+    @staticmethod
+    def forward(ctx, x, p, seed, offset, counter):
+        ctx.save_for_backward(counter)
+        ctx.mask = (p, seed, offset)
+        return _native.dropout_forward(x, p, seed, offset, counter)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        (counter,) = ctx.saved_tensors
+        return _native.dropout_forward(grad, *ctx.mask, counter), None, None, None, None
+
+
+def dropout(x, p, seed, offset=0, counter=None):
+    """x with elements dropped with probability p, the others scaled by 1 / (1 - p); a dropped element is 0 whatever it holds.
+
+    seed, offset: whole numbers that name the mask; equal ones give equal masks.  counter: an int64 tensor of one
+    element beside x that is added to offset when the kernel runs; it must not be written to between a call and its
+    gradient (autograd refuses that).  A step captured into a graph that counts it up draws another mask in each replay."""
+    out = _native.dropout(x, p, seed, offset, counter)
+    return _Dropped.apply(x, p, seed, offset, counter) if out is None else out
+
+
+class Masks:
+    """The masks of a module, one after the other: each is named by the module's seed and the number of the call.
+
+    Calls under a stream capture are numbered on the device, by a counter that the captured work itself
+    counts up, and lie in a range of their own; the module has to be on the device of the rows before."""
+
+    CAPTURED = 1 << 62  # offsets of captured calls begin here
+
+    def _init_masks(self, seed):
+        # of torch's own generator where none is given: torch.manual_seed fixes it, and no two modules share masks
+        self.seed = int(torch.randint(1 << 62, (1,))) if seed is None else int(seed)
+        self.calls = 0
+        self.register_buffer('replays', torch.zeros(1, dtype=torch.int64), persistent=False)
+
+    def _next_mask(self, x):
+        """(seed, offset, counter) of a call on x"""
+        if x.is_cuda and torch.cuda.is_current_stream_capturing():
+            if self.replays.device != x.device:
+                raise RuntimeError("the module is on %s and x on %s: move it there before the capture" % (self.replays.device, x.device))
+            counter = self.replays.clone()
+            self.replays += 1
+            return self.seed, self.CAPTURED, counter
+        self.calls += 1
+        return self.seed, self.calls - 1, None
+
+    def get_extra_state(self):
+        return torch.tensor([self.seed, self.calls], dtype=torch.int64)
+
+    def set_extra_state(self, state):
+        self.seed, self.calls = (int(v) for v in state)
+
+
+class Compressgnn_Dropout(Masks, torch.nn.Module):
+    """dropout(x, p) in training, x itself otherwise.  seed: fixes the masks; its own and the number of calls so far
+    travel with the state dict, so that training resumed from one draws the masks it would have drawn."""
+
+    def __init__(self, p=0.5, seed=None):
+        super().__init__()
+        if not 0 <= p <= 1:
+            raise ValueError("p has to lie in [0, 1], got %r" % (p,))
+        self.p = p
+        self._init_masks(seed)
+
+    def forward(self, x):
+        if not self.training or self.p == 0:
+            return x
+        return dropout(x, self.p, *self._next_mask(x))
+
+    def extra_repr(self):
+        return "p=%g" % self.p

@@ -35,7 +35,9 @@ enum cgnn_status {
     CGNN_EUNSUPPORTED = 4  /* dtype / size outside what the kernels cover         */
 };
 
-enum cgnn_dtype { CGNN_F32 = 0, CGNN_F64 = 1 };
+/* The graph and cluster entry points take CGNN_F32 and CGNN_F64, the row-wise ones (cgnn_layer_norm, cgnn_dropout)
+ * all four. */
+enum cgnn_dtype { CGNN_F32 = 0, CGNN_F64 = 1, CGNN_F16 = 2, CGNN_BF16 = 3 };
 
 /* Which SpMM schedule to run.
  *   ROW: one lane group per row, entries of a row summed in ascending order
@@ -422,6 +424,45 @@ int cgnn_reconstruct_backward_masks(int64_t N, int64_t F, int64_t groups, int64_
                                     const void *grad, const uint32_t *masks, const int32_t *offsets,
                                     const int32_t *perm, const int32_t *sorted_id, void *reps_grad,
                                     void *workspace, size_t workspace_bytes, cgnn_stream_t stream);
+
+/* -------------------------------------------------------- between two layers -- */
+
+/* Layer norm and dropout of node rows.  No counterpart in the reference, whose models take both from torch.
+ *
+ * A cgnn_drop says which elements of a [rows, F] matrix are dropped: element (i, j) is kept where the 16-bit number
+ * drawn for it lies below `kept`, the share of kept elements in 65,536ths (0: none is, 65536: all are).  The numbers
+ * are those of Philox4x32-10 under the key `seed` (low word first), eight a call: call number n = i * ceil(F / 8) + j / 8
+ * has the counter (n low, n high, o low, o high), o = offset + *counter modulo 2^64, and element j % 8 of its
+ * eight is half (j % 8) % 2, the low one first, of word (j % 8) / 2.  So a mask follows from positions alone and is the same in
+ * the gradient and in every type.  counter: device memory that is read when the kernel runs, or NULL: a captured
+ * graph draws another mask in each replay if its program counts it up. */
+typedef struct cgnn_drop {
+    uint64_t seed, offset;
+    const int64_t *counter;
+    int32_t kept;
+} cgnn_drop;
+
+/* out[i,j] = kept ? x[i,j] * 65536 / kept : 0; a dropped element is 0 whatever it holds.  x has rows ldx elements
+ * apart, out is dense.  The gradient is the same call on the output's gradient. */
+int cgnn_dropout(int64_t rows, int64_t F, int dtype, const void *x, int64_t ldx, const cgnn_drop *drop, void *out,
+                 cgnn_stream_t stream);
+
+/* out = drop(relu((x - m) r w + b)), m and v the mean of a row and of its squares around it, r = 1 / sqrt(v + eps);
+ * weight, bias (NULL: 1, 0) of type param_dtype, which is dtype or, for 16-bit rows, CGNN_F32; relu 0: without;
+ * drop NULL: nothing dropped.  stats: [rows, 2], m and r of every row for the gradient, or NULL.  m, v, r and the
+ * value that the ReLU looks at are computed in 64 bits. */
+int cgnn_layer_norm(int64_t rows, int64_t F, int dtype, int param_dtype, const void *x, int64_t ldx, const void *weight,
+                    const void *bias, double eps, int relu, const cgnn_drop *drop, void *out, double *stats,
+                    cgnn_stream_t stream);
+
+/* Its gradients for the same x, weight, bias, relu and drop, rows > 0 and F > 0: dx [rows, F], dweight and dbias [F] of
+ * type param_dtype, each NULL where it is not wanted.  The parameters' sums over the rows have a fixed order; the
+ * workspace is for them and may be NULL where neither is wanted. */
+size_t cgnn_layer_norm_backward_workspace_bytes(int64_t rows, int64_t F, int dtype);
+int cgnn_layer_norm_backward(int64_t rows, int64_t F, int dtype, int param_dtype, const void *grad, int64_t ldg,
+                             const void *x, int64_t ldx, const double *stats, const void *weight, const void *bias, int relu,
+                             const cgnn_drop *drop, void *dx, void *dweight, void *dbias, void *workspace,
+                             size_t workspace_bytes, cgnn_stream_t stream);
 
 /* ---------------------------------------- neighbour sampling on a compressed graph -- */
 
