@@ -75,6 +75,13 @@ struct Draws {
         const uint32_t w = word[i >> 1];
         return (i & 1 ? w >> 16 : w & 0xFFFFu) < kept;
     }
+    // The N that begin at element j of a row come to the front (N divides j).
+    template <int N>
+    __device__ __forceinline__ void from(int j) {
+        const uint32_t w0 = word[0], w1 = word[1], w2 = word[2], w3 = word[3];
+        if constexpr (N <= 4) word[0] = j & 4 ? w2 : w0, word[1] = j & 4 ? w3 : w1;
+        if constexpr (N == 2) word[0] = j & 2 ? word[1] : word[0];
+    }
 };
 
 __device__ __forceinline__ Draws draw(uint64_t seed, uint64_t offset, uint64_t block) {
@@ -131,27 +138,118 @@ __device__ __forceinline__ void store_pack(T *row, int64_t j, int64_t F, const P
 
 // --------------------------------------------------------------------- sums of lanes ----
 
-// The sum over the workgroup's lanes, in every lane: lanes first, then the waves in their order.  `scratch`: one
-// element per wave.
-template <typename A, int THREADS>
-__device__ __forceinline__ A workgroup_sum(A v, A *scratch) {
-#pragma unroll
-    for (int step = 1; step < kWave; step <<= 1) v += __shfl_xor(v, step);
-    if constexpr (THREADS > kWave) {
-        __syncthreads();  // the last sum's readers are done
-        if (threadIdx.x % kWave == 0) scratch[threadIdx.x / kWave] = v;
-        __syncthreads();
-        v = scratch[0];
-#pragma unroll
-        for (int w = 1; w < THREADS / kWave; ++w) v += scratch[w];
-    }
+template <int CONTROL>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CONTROL, 0xF, 0xF, true);
+}
+
+// v of the lane that the step pairs this one with, added to v.  Steps below 16 lanes go through the data-parallel moves
+// of the vector ALU, those of 16 and 32 through its swaps of half rows: none through LDS.
+enum { STEP_XOR1 = 0xB1, STEP_XOR2 = 0x4E, STEP_HALF_MIRROR = 0x141, STEP_MIRROR = 0x140, STEP_ROTATE = 0x120 };
+
+template <int CONTROL>
+__device__ __forceinline__ float add_moved(float v) {
+    return v + __uint_as_float(moved<CONTROL>(__float_as_uint(v)));
+}
+
+template <int CONTROL>
+__device__ __forceinline__ double add_moved(double v) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+    const uint64_t other = (uint64_t)moved<CONTROL>((uint32_t)(bits >> 32)) << 32 | moved<CONTROL>((uint32_t)bits);
+    return v + __builtin_bit_cast(double, other);
+}
+
+template <int LANES>  // 16 or 32
+__device__ __forceinline__ uint32_t swapped(uint32_t v, uint32_t &second) {
+    const auto both = LANES == 16 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    second = both[1];
+    return both[0];
+}
+
+template <int LANES>
+__device__ __forceinline__ float add_swapped(float v) {
+    uint32_t second;
+    const uint32_t first = swapped<LANES>(__float_as_uint(v), second);
+    return __uint_as_float(first) + __uint_as_float(second);
+}
+
+template <int LANES>
+__device__ __forceinline__ double add_swapped(double v) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+    uint32_t low2, high2;
+    const uint32_t low1 = swapped<LANES>((uint32_t)bits, low2), high1 = swapped<LANES>((uint32_t)(bits >> 32), high2);
+    return __builtin_bit_cast(double, (uint64_t)high1 << 32 | low1) + __builtin_bit_cast(double, (uint64_t)high2 << 32 | low2);
+}
+
+// The sum over a lane group (LANES neighbours, a power of two up to a wave), the same bits in each of its lanes.
+template <int LANES, typename A>
+__device__ __forceinline__ A group_sum(A v) {
+    if constexpr (LANES > 1) v = add_moved<STEP_XOR1>(v);
+    if constexpr (LANES > 2) v = add_moved<STEP_XOR2>(v);
+    if constexpr (LANES > 4) v = add_moved<STEP_HALF_MIRROR>(v);
+    if constexpr (LANES > 8) v = add_moved<STEP_MIRROR>(v);
+    if constexpr (LANES > 16) v = add_swapped<16>(v);
+    if constexpr (LANES > 32) v = add_swapped<32>(v);
     return v;
+}
+
+// The sum over the lanes of a wave that have the same place in their groups of LANES.
+template <int LANES, typename A>
+__device__ __forceinline__ A sum_over_groups(A v) {
+    if constexpr (LANES <= 32) v = add_swapped<32>(v);
+    if constexpr (LANES <= 16) v = add_swapped<16>(v);
+    if constexpr (LANES <= 8) v = add_moved<STEP_ROTATE + 8>(v);
+    if constexpr (LANES <= 4) v = add_moved<STEP_ROTATE + 4>(v);
+    if constexpr (LANES <= 2) v = add_moved<STEP_ROTATE + 2>(v);
+    if constexpr (LANES <= 1) v = add_moved<STEP_ROTATE + 1>(v);
+    return v;
+}
+
+// Two sums over the lanes of a row: those of a group, or of the whole workgroup (LANES == THREADS > a wave), whose waves
+// leave theirs in `scratch` (two elements a wave) and add them in their order.
+template <int LANES, int THREADS, typename A>
+__device__ __forceinline__ void row_sums(A &first, A &second, A *scratch) {
+    constexpr int kGroup = LANES < kWave ? LANES : kWave;
+    first = group_sum<kGroup>(first);
+    second = group_sum<kGroup>(second);
+    if constexpr (LANES > kWave) {
+        static_assert(LANES == THREADS, "a row is a lane group's or the whole workgroup's");
+        __syncthreads();  // the last sums' readers are done
+        if (threadIdx.x % kWave == 0) {
+            scratch[threadIdx.x / kWave * 2] = first;
+            scratch[threadIdx.x / kWave * 2 + 1] = second;
+        }
+        __syncthreads();
+        first = scratch[0];
+        second = scratch[1];
+#pragma unroll
+        for (int w = 1; w < THREADS / kWave; ++w) {
+            first += scratch[2 * w];
+            second += scratch[2 * w + 1];
+        }
+    }
 }
 
 // ------------------------------------------------------------------------ layer norm ----
 
-// 1 / sqrt(a).
-__device__ __forceinline__ double reciprocal_root(double a) { return 1.0 / __builtin_sqrt(a); }
+// 1 / sqrt(a): the hardware's estimate of half the bits, and two steps of Newton's method for 1 / r^2 = a.
+__device__ __forceinline__ double reciprocal_root(double a) {
+    double r = __builtin_amdgcn_rsq(a);
+#pragma unroll
+    for (int step = 0; step < 2; ++step) r = __builtin_fma(0.5 * r, __builtin_fma(-a * r, r, 1.0), r);
+    return a < __builtin_inf() ? r : a - a;  // of an infinite one 0 in mathematics; no row with finite differences has it
+}
+
+// Mean and variance of a row from sums over its differences to one of its own elements: that element is at most sqrt(F)
+// deviations from the mean, so what the last step takes away leaves at least 1 / F of the squares.
+// One reading of the row does, and nothing is lost on an offset, however large.
+struct Moments {
+    double mean, variance;
+};
+__device__ __forceinline__ Moments moments(double pivot, double sum, double squares, double inverse_F) {
+    const double shift = sum * inverse_F, variance = __builtin_fma(-shift, shift, squares * inverse_F);
+    return {pivot + shift, variance < 0 ? 0 : variance};
+}
 
 // A parameter of the rows' type or of float (`wide`); 1 or 0 where there is none.
 template <typename T>
@@ -163,6 +261,9 @@ struct Params {
         return wide ? (compute_t<T>)static_cast<const float *>(data)[j] : (compute_t<T>)static_cast<const T *>(data)[j];
     }
 };
+
+__device__ __forceinline__ float fused(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+__device__ __forceinline__ double fused(double a, double b, double c) { return __builtin_fma(a, b, c); }
 
 template <typename T>
 struct NormArgs {
@@ -181,9 +282,71 @@ struct NormArgs {
     int64_t rows, F;
 };
 
-// h * w + b in 64 bits, by the one expression that both passes use.
-__device__ __forceinline__ double before_relu(double x, double mean, double rstd, double w, double b) {
-    return __builtin_fma((x - mean) * rstd, w, b);
+// What the ReLU sees of elements i = 0 ... N - 1: v = h w + b with h = (x - m) r, h in `h` too.  Forward pass and
+// gradient call this with the same numbers, and the side of zero that v is on is that of its value in 64 bits:
+// h is rounded once and h w + b once, so v is less than 2^-24 (|b| + 2 |v|) off and its sign is certain where |v| > 2^-21 |b|;
+// the few elements in between (one of a million, and those that are 0) are computed again.  A float decision alone would let
+// a sum of a million elements differ by a whole gradient now and then.
+template <int N, typename T, typename C>
+__device__ __forceinline__ void normalised(const T (&x)[N], double mean, double rstd, const C (&w)[N], const C (&b)[N], bool relu,
+                                           C (&h)[N], C (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        h[i] = (C)(((double)x[i] - mean) * rstd);
+        v[i] = fused(h[i], w[i], b[i]);
+    }
+    if constexpr (sizeof(C) == 4) {
+        if (!relu) return;
+        bool unsure = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) unsure = unsure || __builtin_fabsf(v[i]) <= __builtin_fabsf(b[i]) * 0x1p-21f;
+        if (unsure)
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (__builtin_fabsf(v[i]) <= __builtin_fabsf(b[i]) * 0x1p-21f) {
+                    float weight = w[i], bias = b[i];
+                    asm volatile("" : "+v"(weight), "+v"(bias));  // widened here: not ahead of the rows, in registers of its own
+                    v[i] = (C)__builtin_fma(((double)x[i] - mean) * rstd, (double)weight, (double)bias);
+                }
+    }
+}
+
+constexpr int64_t kMostPacks = 2048;  // of 16 bytes: longer rows do not fit the registers of a workgroup
+
+// How a row is spread: packs of 16 bytes over `lanes` lanes, `packs` on each; a workgroup has `threads`.  0 lanes:
+// more packs than most_packs.
+struct RowShape {
+    int lanes, packs, threads;
+};
+
+inline RowShape row_shape(int64_t F, size_t element, int64_t most_packs) {
+    const int64_t packs = ceil_div(F, 16 / (int64_t)element);
+    if (packs > most_packs) return {0, 0, 1024};
+    if (packs <= 64) return {pow2_ceil(packs), 1, kBlock};
+    if (packs <= 128) return {64, 2, kBlock};
+    if (packs <= 512) return {256, packs <= 256 ? 1 : 2, 256};
+    return {1024, packs <= 1024 ? 1 : 2, 1024};
+}
+
+template <int LANES, int PACKS, int THREADS>
+struct ShapeTag {
+    static constexpr int lanes = LANES, packs = PACKS, threads = THREADS;
+};
+
+// Calls `run` with the tag of a shape of at least one lane.
+template <typename F>
+int with_row_shape(const RowShape &s, F &&run) {
+    switch (s.lanes) {
+        case 1: return run(ShapeTag<1, 1, kBlock>());
+        case 2: return run(ShapeTag<2, 1, kBlock>());
+        case 4: return run(ShapeTag<4, 1, kBlock>());
+        case 8: return run(ShapeTag<8, 1, kBlock>());
+        case 16: return run(ShapeTag<16, 1, kBlock>());
+        case 32: return run(ShapeTag<32, 1, kBlock>());
+        case 64: return s.packs == 1 ? run(ShapeTag<64, 1, kBlock>()) : run(ShapeTag<64, 2, kBlock>());
+        case 256: return s.packs == 1 ? run(ShapeTag<256, 1, 256>()) : run(ShapeTag<256, 2, 256>());
+        default: return s.packs == 1 ? run(ShapeTag<1024, 1, 1024>()) : run(ShapeTag<1024, 2, 1024>());
+    }
 }
 
 }  // namespace cgnn
