@@ -13,10 +13,6 @@ constexpr int kLongParts = 512;
 constexpr int kLanes = 64;      // ... lanes side by side, kDrawn columns each
 constexpr int kChain = 512;     // other rows: as many of them at most are added up one after the other by a lane, in float
 
-// Of 16-bit rows a lane has eight columns in a pack, and in float their sums, parameters and values: two packs a lane are beyond
-// the 128 registers of a workgroup of 1,024.
-RowShape gradient_shape(int64_t F, size_t element) { return row_shape(F, element, element == 2 ? kMostPacks / 2 : kMostPacks); }
-
 int64_t long_rows(int64_t rows) { return std::max<int64_t>(kLongRows, ceil_div(rows, kLongParts)); }
 
 // Workgroups of norm_gradients_kernel, each of which leaves a part of the parameters' sums: as many as are resident, more
@@ -26,14 +22,11 @@ int64_t row_parts(int64_t rows, const RowShape &s) {
     return std::max(std::min<int64_t>(tiles, 256 * 1024 / s.threads), ceil_div(tiles, kChain));
 }
 
-int64_t parts_of(int64_t rows, int64_t F, size_t element) {
-    const RowShape shape = gradient_shape(F, element);
-    return shape.lanes ? row_parts(rows, shape) : ceil_div(rows, long_rows(rows));
-}
+int64_t long_parts(int64_t rows) { return ceil_div(rows, long_rows(rows)); }
 
 // Rows that fit the registers of their lanes, as in the forward pass: x and the gradient are read once for dx and for
 // the parameters' sums, which every lane holds for its own columns until its rows are through.
-template <typename T, int LANES, int K, int THREADS, bool DROP>
+template <typename T, int LANES, int K, int THREADS, bool RELU, bool DROP>
 __global__ __launch_bounds__(THREADS) void norm_gradients_kernel(NormArgs<T> a) {
     using C = compute_t<T>;
     constexpr int N = 16 / (int)sizeof(T), GROUPS = THREADS / LANES, WAVES = THREADS / kWave;
@@ -41,42 +34,52 @@ __global__ __launch_bounds__(THREADS) void norm_gradients_kernel(NormArgs<T> a) 
     __shared__ C scratch[LANES > kWave ? WAVES * 2 : WAVES * COLUMNS];
     const int lane = threadIdx.x % LANES, F = (int)a.F;
     const int64_t step = (int64_t)gridDim.x * GROUPS;
+    const int64_t extent_x = (a.rows - 1) * a.ldx + F, extent_g = (a.rows - 1) * a.ldg + F;
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
     const C inverse_F = C(1) / (C)F;
     int64_t r = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LANES;
 
-    Pack<T, N> next_x[K], next_g[K];
+    words_t next_x[K], next_g[K];
     double next_mean = 0, next_rstd = 0;
     auto ask = [&](int64_t row) {
         next_mean = a.stats[2 * row];
         next_rstd = a.stats[2 * row + 1];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int j = (lane + k * LANES) * N;
-            next_x[k] = load_pack<T, N>(a.x + row * a.ldx, j, F);
-            next_g[k] = load_pack<T, N>(a.grad + row * a.ldg, j, F);
+            const int j = (lane + k * LANES) * N, from = j < F ? j : 0;
+            next_x[k] = ask_within<T>(a.x, row * a.ldx + from, extent_x);
+            next_g[k] = ask_within<T>(a.grad, row * a.ldg + from, extent_g);
         }
     };
     if (r < a.rows) ask(r);
     C w[K][N], b[K][N], dw[K][N], db[K][N];
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k) {
+        a.weight.template read<N>((lane + k * LANES) * N, F, C(1), w[k]);
+        if constexpr (RELU) a.bias.template read<N>((lane + k * LANES) * N, F, C(0), b[k]);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int j = (lane + k * LANES) * N + i;
-            w[k][i] = j < F ? a.weight.at(j, C(1)) : C(0);
-            b[k][i] = j < F && a.relu ? a.bias.at(j, C(0)) : C(0);
+            if constexpr (!RELU) b[k][i] = C(0);
             dw[k][i] = db[k][i] = C(0);
         }
+    }
+    arrived(next_x);
+    arrived(next_g);
+    arrived(next_mean);
+    arrived(next_rstd);
+    arrived(w);
+    arrived(b);
     for (; r < a.rows; r += step) {
         C h[K][N], g[K][N];
-        const double mean = next_mean, rstd = next_rstd;
+        const Centre<C> centre(next_mean, next_rstd);
         C sum = 0, product = 0;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int j = (lane + k * LANES) * N;
+            const int j = (lane + k * LANES) * N, from = j < F ? j : 0;
+            const auto x = settled<T>(next_x[k], a.x, r * a.ldx + from, extent_x);
+            const auto d = settled<T>(next_g[k], a.grad, r * a.ldg + from, extent_g);
             C v[N];
-            normalised<N>(next_x[k].v, mean, rstd, w[k], b[k], a.relu, h[k], v);
+            normalised<RELU, N>(x.v, centre, w[k], b[k], h[k], v);
             Draws drawn;
             if constexpr (DROP) {
                 drawn = draw(a.drop.seed, offset, (uint64_t)(r * a.drop.blocks + j / kDrawn));
@@ -84,12 +87,17 @@ __global__ __launch_bounds__(THREADS) void norm_gradients_kernel(NormArgs<T> a) 
             }
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                C d = (C)next_g[k].v[i];
-                if constexpr (DROP) d = drawn.keeps(i, a.drop.kept) ? d * (C)a.drop.scale : C(0);
-                g[k][i] = a.relu && v[i] <= 0 ? C(0) : d;
+                C c = (C)d.v[i];
+                if constexpr (DROP) c = drawn.keeps(i, a.drop.kept) ? c * (C)a.drop.scale : C(0);
+                if constexpr (RELU) c = v[i] <= 0 ? C(0) : c;
+                g[k][i] = c;
             }
+            if (j + N > F)  // behind the row's end lies what the next one holds
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (j + i >= F) h[k][i] = g[k][i] = C(0);
         }
-        if (r + step < a.rows) ask(r + step);
+        ask(r + step < a.rows ? r + step : r);
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -103,14 +111,19 @@ __global__ __launch_bounds__(THREADS) void norm_gradients_kernel(NormArgs<T> a) 
         if (a.dx) {
             row_sums<LANES, THREADS>(sum, product, scratch);
             const C c1 = sum * inverse_F, c2 = product * inverse_F;
+            Pack<T, N> dx[K];
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                const int j = (lane + k * LANES) * N;
-                Pack<T, N> dx;
 #pragma unroll
-                for (int i = 0; i < N; ++i) dx.v[i] = (T)((C)rstd * (fused(-h[k][i], c2, g[k][i]) - c1));
-                if (j < F) store_pack<T, N>(a.dx + r * a.F, j, F, dx);
+                for (int i = 0; i < N; ++i) g[k][i] = centre.scale * (fused(-h[k][i], c2, g[k][i]) - c1);
+                dx[k] = rounded<T, N>(g[k]);
             }
+            arrived(next_x);
+            arrived(next_g);
+            arrived(next_mean);
+            arrived(next_rstd);
+#pragma unroll
+            for (int k = 0; k < K; ++k) store_columns<T, N>(a.dx + r * a.F, (lane + k * LANES) * N, F, dx[k]);
         }
     }
     if (a.partial == nullptr) return;
@@ -148,42 +161,40 @@ __global__ __launch_bounds__(THREADS) void norm_gradients_kernel(NormArgs<T> a) 
 }
 
 // Eight elements of a row as the gradient sees them: h, and g as described above.
-template <typename T, bool DROP>
-__device__ __forceinline__ void masked(const NormArgs<T> &a, int64_t r, int64_t j, double mean, double rstd, uint64_t offset,
+template <typename T, bool RELU, bool DROP>
+__device__ __forceinline__ void masked(const NormArgs<T> &a, int64_t r, int64_t j, const Centre<compute_t<T>> &centre, uint64_t offset,
                                        compute_t<T> (&w)[kDrawn], compute_t<T> (&h)[kDrawn], compute_t<T> (&g)[kDrawn]) {
     using C = compute_t<T>;
     const auto x = load_pack<T, kDrawn>(a.x + r * a.ldx, j, a.F);
     const auto d = load_pack<T, kDrawn>(a.grad + r * a.ldg, j, a.F);
-    C b[kDrawn], v[kDrawn];
-#pragma unroll
-    for (int i = 0; i < kDrawn; ++i) {
-        w[i] = j + i < a.F ? a.weight.at(j + i, C(1)) : C(0);
-        b[i] = j + i < a.F && a.relu ? a.bias.at(j + i, C(0)) : C(0);
-    }
-    normalised<kDrawn>(x.v, mean, rstd, w, b, a.relu, h, v);
+    C b[kDrawn] = {}, v[kDrawn];
+    a.weight.template read<kDrawn>(j, a.F, C(1), w);
+    if constexpr (RELU) a.bias.template read<kDrawn>(j, a.F, C(0), b);
+    normalised<RELU, kDrawn>(x.v, centre, w, b, h, v);
     Draws drawn;
     if constexpr (DROP) drawn = draw(a.drop.seed, offset, (uint64_t)(r * a.drop.blocks + j / kDrawn));
 #pragma unroll
     for (int i = 0; i < kDrawn; ++i) {
         C c = (C)d.v[i];
         if constexpr (DROP) c = drawn.keeps(i, a.drop.kept) ? c * (C)a.drop.scale : C(0);
-        g[i] = a.relu && v[i] <= 0 ? C(0) : c;
+        if constexpr (RELU) c = v[i] <= 0 ? C(0) : c;
+        g[i] = c;
     }
 }
 
 constexpr int kLongThreads = 1024;
 
 // dx of longer rows: a workgroup per row, which reads it twice.
-template <typename T, bool DROP>
+template <typename T, bool RELU, bool DROP>
 __global__ __launch_bounds__(kLongThreads) void norm_long_dx_kernel(NormArgs<T> a) {
     using C = compute_t<T>;
     __shared__ C scratch[kLongThreads / kWave * 2];
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const double mean = a.stats[2 * r], rstd = a.stats[2 * r + 1];
+        const Centre<C> centre(a.stats[2 * r], a.stats[2 * r + 1]);
         C sum = 0, product = 0, w[kDrawn], h[kDrawn], g[kDrawn];
         for (int64_t j = (int64_t)threadIdx.x * kDrawn; j < a.F; j += (int64_t)kLongThreads * kDrawn) {
-            masked<T, DROP>(a, r, j, mean, rstd, offset, w, h, g);
+            masked<T, RELU, DROP>(a, r, j, centre, offset, w, h, g);
 #pragma unroll
             for (int i = 0; i < kDrawn; ++i) {
                 sum = fused(g[i], w[i], sum);
@@ -193,17 +204,17 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_dx_kernel(NormArgs<T> 
         row_sums<kLongThreads, kLongThreads>(sum, product, scratch);
         const C c1 = sum / (C)a.F, c2 = product / (C)a.F;
         for (int64_t j = (int64_t)threadIdx.x * kDrawn; j < a.F; j += (int64_t)kLongThreads * kDrawn) {
-            masked<T, DROP>(a, r, j, mean, rstd, offset, w, h, g);
-            Pack<T, kDrawn> dx;
+            masked<T, RELU, DROP>(a, r, j, centre, offset, w, h, g);
+            C dx[kDrawn];
 #pragma unroll
-            for (int i = 0; i < kDrawn; ++i) dx.v[i] = (T)((C)rstd * (fused(-h[i], c2, g[i] * w[i]) - c1));
-            store_pack<T, kDrawn>(a.dx + r * a.F, j, a.F, dx);
+            for (int i = 0; i < kDrawn; ++i) dx[i] = centre.scale * (fused(-h[i], c2, g[i] * w[i]) - c1);
+            store_pack<T, kDrawn>(a.dx + r * a.F, j, a.F, rounded<T, kDrawn>(dx));
         }
     }
 }
 
 // Their dw and db: blockIdx.x names the part, `part` rows each, blockIdx.y the columns.
-template <typename T, bool DROP>
+template <typename T, bool RELU, bool DROP>
 __global__ __launch_bounds__(kBlock) void norm_long_parts_kernel(NormArgs<T> a, int64_t part) {
     using C = compute_t<T>;
     __shared__ C sums[kBlock / kLanes][2][kDrawn][kLanes];
@@ -215,7 +226,7 @@ __global__ __launch_bounds__(kBlock) void norm_long_parts_kernel(NormArgs<T> a, 
     if (j < a.F)
         for (int64_t r = (int64_t)blockIdx.x * part + group; r < last; r += kBlock / kLanes) {
             C w[kDrawn], h[kDrawn], g[kDrawn];
-            masked<T, DROP>(a, r, j, a.stats[2 * r], a.stats[2 * r + 1], offset, w, h, g);
+            masked<T, RELU, DROP>(a, r, j, Centre<C>(a.stats[2 * r], a.stats[2 * r + 1]), offset, w, h, g);
 #pragma unroll
             for (int i = 0; i < kDrawn; ++i) {
                 dw[i] = fused(g[i], h[i], dw[i]);
@@ -244,71 +255,73 @@ __global__ __launch_bounds__(kBlock) void norm_long_parts_kernel(NormArgs<T> a, 
             }
 }
 
-// The parts' sums, added up in 64 bits in the order of the parts: column c < F of the weight's gradient, then the bias's.
+// The parts' sums, added up in 64 bits in an order that the number of parts fixes: column c < F of the weight's gradient, then
+// the bias's.  Sixteen columns a workgroup: as many lines of 64 bytes in flight as it has lane groups.
+constexpr int kSumColumns = 16, kSumThreads = 1024, kSumUnroll = 4;
+
 template <typename C, typename P>
-__global__ __launch_bounds__(kBlock) void norm_sum_parts_kernel(const C *partial, int64_t parts, int64_t F, P *dweight, P *dbias) {
-    constexpr int kColumns = 16, kGroups = kBlock / kColumns;
-    __shared__ double sums[kGroups][kColumns];
-    const int lane = threadIdx.x % kColumns, group = threadIdx.x / kColumns;
-    const int64_t c = (int64_t)blockIdx.x * kColumns + lane;
+__global__ __launch_bounds__(kSumThreads) void norm_sum_parts_kernel(const C *partial, int64_t parts, int64_t F, P *dweight, P *dbias) {
+    constexpr int GROUPS = kSumThreads / kSumColumns;
+    __shared__ double sums[GROUPS][kSumColumns];
+    const int lane = threadIdx.x % kSumColumns, group = threadIdx.x / kSumColumns;
+    const int64_t c = (int64_t)blockIdx.x * kSumColumns + lane;
     double sum = 0;
     if (c < 2 * F)
-        for (int64_t k = group; k < parts; k += kGroups) sum += (double)partial[k * 2 * F + c];
-    sums[group][lane] = sum;
-    __syncthreads();
-    if (group != 0 || c >= 2 * F) return;
+        for (int64_t k = group; k < parts; k += GROUPS * kSumUnroll) {
+            C part[kSumUnroll];
 #pragma unroll
-    for (int k = 1; k < kGroups; ++k) sum += sums[k][lane];
+            for (int u = 0; u < kSumUnroll; ++u) part[u] = k + u * GROUPS < parts ? partial[(k + u * GROUPS) * 2 * F + c] : C(0);
+#pragma unroll
+            for (int u = 0; u < kSumUnroll; ++u) sum += (double)part[u];
+        }
+    sums[group][lane] = sum;
+#pragma unroll
+    for (int half = GROUPS / 2; half > 0; half /= 2) {
+        __syncthreads();
+        if (group < half) sums[group][lane] += sums[group + half][lane];
+    }
+    if (group != 0 || c >= 2 * F) return;
     P *to = c < F ? dweight : dbias;
-    if (to) to[c < F ? c : c - F] = (P)(compute_t<P>)sum;
+    if (to) to[c < F ? c : c - F] = (P)(compute_t<P>)sums[0][lane];
+}
+
+template <typename T, bool RELU, bool DROP>
+int gradients_launch(const NormArgs<T> &a, const RowShape &shape, int64_t parts, hipStream_t stream) {
+    if (shape.lanes)
+        return with_row_shape<T>(shape, [&](auto tag) {
+            using S = decltype(tag);
+            hipLaunchKernelGGL((norm_gradients_kernel<T, S::lanes, S::packs, S::threads, RELU, DROP>), dim3((unsigned)parts), dim3(S::threads),
+                               0, stream, a);
+            return check_launch("layer_norm_backward");
+        });
+    if (a.dx) {
+        hipLaunchKernelGGL((norm_long_dx_kernel<T, RELU, DROP>), dim3((unsigned)std::min<int64_t>(a.rows, 1024)), dim3(kLongThreads), 0, stream, a);
+        if (int rc = check_launch("layer_norm_backward")) return rc;
+    }
+    if (a.partial) {
+        const dim3 grid((unsigned)parts, (unsigned)ceil_div(a.F, (int64_t)kLanes * kDrawn));
+        hipLaunchKernelGGL((norm_long_parts_kernel<T, RELU, DROP>), grid, dim3(kBlock), 0, stream, a, long_rows(a.rows));
+    }
+    return check_launch("layer_norm_backward");
 }
 
 template <typename T>
 int norm_backward_typed(NormArgs<T> a, bool drops, int param_dtype, void *dweight, void *dbias, hipStream_t stream) {
     using C = compute_t<T>;
-    const RowShape shape = gradient_shape(a.F, sizeof(T));
-    const int64_t parts = parts_of(a.rows, a.F, sizeof(T));
+    RowShape shape = row_shape(a.F, sizeof(T));
+    if (!loads_whole(a.rows, a.F, a.ldx, sizeof(T)) || !loads_whole(a.rows, a.F, a.ldg, sizeof(T))) shape.lanes = 0;
+    const int64_t parts = shape.lanes ? row_parts(a.rows, shape) : long_parts(a.rows);
     const bool sums = dweight != nullptr || dbias != nullptr;
     if (!sums) a.partial = nullptr;
-    int rc = CGNN_OK;
-    if (shape.lanes) {
-        rc = with_row_shape(shape, [&](auto tag) {
-            using S = decltype(tag);
-            if constexpr (S::lanes * S::packs * (int)sizeof(T) < 2 * 2048 || sizeof(T) > 2) {
-                const dim3 grid((unsigned)parts);
-                if (drops)
-                    hipLaunchKernelGGL((norm_gradients_kernel<T, S::lanes, S::packs, S::threads, true>), grid, dim3(S::threads), 0, stream, a);
-                else
-                    hipLaunchKernelGGL((norm_gradients_kernel<T, S::lanes, S::packs, S::threads, false>), grid, dim3(S::threads), 0, stream, a);
-            }
-            return check_launch("layer_norm_backward");
-        });
-    } else {
-        if (a.dx) {
-            const dim3 grid((unsigned)std::min<int64_t>(a.rows, 1024));
-            if (drops)
-                hipLaunchKernelGGL((norm_long_dx_kernel<T, true>), grid, dim3(kLongThreads), 0, stream, a);
-            else
-                hipLaunchKernelGGL((norm_long_dx_kernel<T, false>), grid, dim3(kLongThreads), 0, stream, a);
-            rc = check_launch("layer_norm_backward");
-        }
-        if (rc == CGNN_OK && sums) {
-            const int64_t part = long_rows(a.rows);
-            const dim3 grid((unsigned)parts, (unsigned)ceil_div(a.F, (int64_t)kLanes * kDrawn));
-            if (drops)
-                hipLaunchKernelGGL((norm_long_parts_kernel<T, true>), grid, dim3(kBlock), 0, stream, a, part);
-            else
-                hipLaunchKernelGGL((norm_long_parts_kernel<T, false>), grid, dim3(kBlock), 0, stream, a, part);
-            rc = check_launch("layer_norm_backward");
-        }
-    }
+    const int rc = drops ? (a.relu ? gradients_launch<T, true, true>(a, shape, parts, stream) : gradients_launch<T, false, true>(a, shape, parts, stream))
+                         : (a.relu ? gradients_launch<T, true, false>(a, shape, parts, stream) : gradients_launch<T, false, false>(a, shape, parts, stream));
     if (rc != CGNN_OK || !sums) return rc;
-    const dim3 columns((unsigned)ceil_div(2 * a.F, 16));
+    const dim3 columns((unsigned)ceil_div(2 * a.F, kSumColumns));
     if (param_dtype == CGNN_F32)
-        hipLaunchKernelGGL((norm_sum_parts_kernel<C, float>), columns, dim3(kBlock), 0, stream, a.partial, parts, a.F,
+        hipLaunchKernelGGL((norm_sum_parts_kernel<C, float>), columns, dim3(kSumThreads), 0, stream, a.partial, parts, a.F,
                            static_cast<float *>(dweight), static_cast<float *>(dbias));
     else
-        hipLaunchKernelGGL((norm_sum_parts_kernel<C, T>), columns, dim3(kBlock), 0, stream, a.partial, parts, a.F,
+        hipLaunchKernelGGL((norm_sum_parts_kernel<C, T>), columns, dim3(kSumThreads), 0, stream, a.partial, parts, a.F,
                            static_cast<T *>(dweight), static_cast<T *>(dbias));
     return check_launch("layer_norm_backward");
 }
@@ -320,7 +333,9 @@ using namespace cgnn;
 
 extern "C" size_t cgnn_layer_norm_backward_workspace_bytes(int64_t rows, int64_t F, int dtype) {
     if (rows <= 0 || F <= 0) return 0;
-    return (size_t)parts_of(rows, F, row_type_bytes(dtype)) * 2 * (size_t)F * (dtype == CGNN_F64 ? 8 : 4);
+    const RowShape shape = row_shape(F, row_type_bytes(dtype));
+    const int64_t parts = std::max(long_parts(rows), shape.lanes ? row_parts(rows, shape) : 0);  // rows that lie too close take the other way
+    return (size_t)parts * 2 * (size_t)F * (dtype == CGNN_F64 ? 8 : 4);
 }
 
 extern "C" int cgnn_layer_norm_backward(int64_t rows, int64_t F, int dtype, int param_dtype, const void *grad, int64_t ldg,

@@ -8,48 +8,53 @@ namespace {
 
 // Rows that fit the registers of their lanes: LANES of them hold K packs of 16 bytes each, so a row is read once and
 // written once.  The packs of the next row are asked for before this one's are used.
-template <typename T, int LANES, int K, int THREADS, bool DROP>
+template <typename T, int LANES, int K, int THREADS, bool RELU, bool DROP>
 __global__ __launch_bounds__(THREADS) void norm_rows_kernel(NormArgs<T> a) {
     using C = compute_t<T>;
     constexpr int N = 16 / (int)sizeof(T), GROUPS = THREADS / LANES;
     __shared__ double scratch[LANES > kWave ? THREADS / kWave * 2 : 1];
     const int lane = threadIdx.x % LANES, F = (int)a.F;
-    const int64_t step = (int64_t)gridDim.x * GROUPS;
+    const int64_t step = (int64_t)gridDim.x * GROUPS, extent = (a.rows - 1) * a.ldx + F;
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
     const double inverse_F = 1.0 / (double)F;
     int64_t r = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LANES;
 
-    Pack<T, N> next[K];
+    words_t next[K];
     T next_first = T(0);
     auto ask = [&](int64_t row) {
-        const T *x = a.x + row * a.ldx;
-        next_first = x[0];
+        const int64_t at = row * a.ldx;
+        next_first = a.x[at];
 #pragma unroll
-        for (int k = 0; k < K; ++k) next[k] = load_pack<T, N>(x, (lane + k * LANES) * N, F);
+        for (int k = 0; k < K; ++k) {
+            const int j = (lane + k * LANES) * N;
+            next[k] = ask_within<T>(a.x, at + (j < F ? j : 0), extent);
+        }
     };
     if (r < a.rows) ask(r);
     C w[K][N], b[K][N];
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int j = (lane + k * LANES) * N + i;
-            w[k][i] = j < F ? a.weight.at(j, C(1)) : C(0);
-            b[k][i] = j < F ? a.bias.at(j, C(0)) : C(0);
-        }
+    for (int k = 0; k < K; ++k) {
+        a.weight.template read<N>((lane + k * LANES) * N, F, C(1), w[k]);
+        a.bias.template read<N>((lane + k * LANES) * N, F, C(0), b[k]);
+    }
+    arrived(next);
+    arrived(next_first);
+    arrived(w);
+    arrived(b);
     for (; r < a.rows; r += step) {
         Pack<T, N> x[K];
-        const double pivot = (double)next_first;
+        const T first = next_first;
+        const double pivot = (double)first;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            x[k] = next[k];
             const int j = (lane + k * LANES) * N;
+            x[k] = settled<T>(next[k], a.x, r * a.ldx + (j < F ? j : 0), extent);
             if (j + N > F)  // what lies behind the row's end adds nothing to its sums
 #pragma unroll
                 for (int i = 0; i < N; ++i)
-                    if (j + i >= F) x[k].v[i] = next_first;
+                    if (j + i >= F) x[k].v[i] = first;
         }
-        if (r + step < a.rows) ask(r + step);
+        ask(r + step < a.rows ? r + step : r);
         double sum = 0, squares = 0;
 #pragma unroll
         for (int k = 0; k < K; ++k)
@@ -61,18 +66,14 @@ __global__ __launch_bounds__(THREADS) void norm_rows_kernel(NormArgs<T> a) {
             }
         row_sums<LANES, THREADS>(sum, squares, scratch);
         const Moments m = moments(pivot, sum, squares, inverse_F);
-        const double rstd = reciprocal_root(m.variance + a.eps);
-        if (a.stats && lane == 0) {
-            a.stats[2 * r] = m.mean;
-            a.stats[2 * r + 1] = rstd;
-        }
+        const Centre<C> centre(m.mean, reciprocal_root(m.variance + a.eps));
         T *out = a.out + r * a.F;
+        Pack<T, N> y[K];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int j = (lane + k * LANES) * N;
-            Pack<T, N> y;
             C h[N], v[N];
-            normalised<N>(x[k].v, m.mean, rstd, w[k], b[k], a.relu, h, v);
+            normalised<RELU, N>(x[k].v, centre, w[k], b[k], h, v);
             Draws drawn;
             if constexpr (DROP) {
                 drawn = draw(a.drop.seed, offset, (uint64_t)(r * a.drop.blocks + j / kDrawn));
@@ -80,19 +81,26 @@ __global__ __launch_bounds__(THREADS) void norm_rows_kernel(NormArgs<T> a) {
             }
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                C c = a.relu && v[i] <= 0 ? C(0) : v[i];
-                if constexpr (DROP) c = drawn.keeps(i, a.drop.kept) ? c * (C)a.drop.scale : C(0);
-                y.v[i] = (T)c;
+                if constexpr (RELU) v[i] = v[i] <= 0 ? C(0) : v[i];
+                if constexpr (DROP) v[i] = drawn.keeps(i, a.drop.kept) ? v[i] * (C)a.drop.scale : C(0);
             }
-            if (j < F) store_pack<T, N>(out, j, F, y);
+            y[k] = rounded<T, N>(v);
         }
+        arrived(next);
+        arrived(next_first);
+        if (a.stats && lane == 0) {
+            a.stats[2 * r] = centre.mean;
+            a.stats[2 * r + 1] = centre.rstd;
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) store_columns<T, N>(out, (lane + k * LANES) * N, F, y[k]);
     }
 }
 
 // Longer rows: a workgroup a row, which reads it twice.
 constexpr int kLongThreads = 1024;
 
-template <typename T, bool DROP>
+template <typename T, bool RELU, bool DROP>
 __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs<T> a) {
     using C = compute_t<T>;
     __shared__ double scratch[kLongThreads / kWave * 2];
@@ -113,52 +121,40 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs<T> a) 
         }
         row_sums<kLongThreads, kLongThreads>(sum, squares, scratch);
         const Moments m = moments(pivot, sum, squares, 1.0 / (double)a.F);
-        const double rstd = reciprocal_root(m.variance + a.eps);
+        const Centre<C> centre(m.mean, reciprocal_root(m.variance + a.eps));
         if (a.stats && threadIdx.x == 0) {
-            a.stats[2 * r] = m.mean;
-            a.stats[2 * r + 1] = rstd;
+            a.stats[2 * r] = centre.mean;
+            a.stats[2 * r + 1] = centre.rstd;
         }
         for (int64_t j = (int64_t)threadIdx.x * kDrawn; j < a.F; j += (int64_t)kLongThreads * kDrawn) {
             const auto p = load_pack<T, kDrawn>(x, j, a.F);
-            Pack<T, kDrawn> y;
             C w[kDrawn], b[kDrawn], h[kDrawn], v[kDrawn];
-#pragma unroll
-            for (int i = 0; i < kDrawn; ++i) {
-                w[i] = j + i < a.F ? a.weight.at(j + i, C(1)) : C(0);
-                b[i] = j + i < a.F ? a.bias.at(j + i, C(0)) : C(0);
-            }
-            normalised<kDrawn>(p.v, m.mean, rstd, w, b, a.relu, h, v);
+            a.weight.template read<kDrawn>(j, a.F, C(1), w);
+            a.bias.template read<kDrawn>(j, a.F, C(0), b);
+            normalised<RELU, kDrawn>(p.v, centre, w, b, h, v);
             Draws drawn;
             if constexpr (DROP) drawn = draw(a.drop.seed, offset, (uint64_t)(r * a.drop.blocks + j / kDrawn));
 #pragma unroll
             for (int i = 0; i < kDrawn; ++i) {
-                C c = a.relu && v[i] <= 0 ? C(0) : v[i];
-                if constexpr (DROP) c = drawn.keeps(i, a.drop.kept) ? c * (C)a.drop.scale : C(0);
-                y.v[i] = (T)c;
+                if constexpr (RELU) v[i] = v[i] <= 0 ? C(0) : v[i];
+                if constexpr (DROP) v[i] = drawn.keeps(i, a.drop.kept) ? v[i] * (C)a.drop.scale : C(0);
             }
-            store_pack<T, kDrawn>(out, j, a.F, y);
+            store_pack<T, kDrawn>(out, j, a.F, rounded<T, kDrawn>(v));
         }
     }
 }
 
-template <typename T>
-int norm_typed(const NormArgs<T> &a, bool drops, hipStream_t stream) {
-    const RowShape shape = row_shape(a.F, sizeof(T), kMostPacks);
-    if (shape.lanes == 0) {
-        const dim3 grid((unsigned)std::min<int64_t>(a.rows, 1024));
-        if (drops)
-            hipLaunchKernelGGL((norm_long_kernel<T, true>), grid, dim3(kLongThreads), 0, stream, a);
-        else
-            hipLaunchKernelGGL((norm_long_kernel<T, false>), grid, dim3(kLongThreads), 0, stream, a);
+template <typename T, bool RELU, bool DROP>
+int norm_launch(const NormArgs<T> &a, hipStream_t stream) {
+    const RowShape shape = row_shape(a.F, sizeof(T));
+    if (shape.lanes == 0 || !loads_whole(a.rows, a.F, a.ldx, sizeof(T))) {
+        hipLaunchKernelGGL((norm_long_kernel<T, RELU, DROP>), dim3((unsigned)std::min<int64_t>(a.rows, 1024)), dim3(kLongThreads), 0, stream, a);
         return check_launch("layer_norm");
     }
-    return with_row_shape(shape, [&](auto tag) {
+    return with_row_shape<T>(shape, [&](auto tag) {
         using S = decltype(tag);
         const dim3 grid((unsigned)std::min<int64_t>(ceil_div(a.rows, S::threads / S::lanes), 256 * 2048 / S::threads));
-        if (drops)
-            hipLaunchKernelGGL((norm_rows_kernel<T, S::lanes, S::packs, S::threads, true>), grid, dim3(S::threads), 0, stream, a);
-        else
-            hipLaunchKernelGGL((norm_rows_kernel<T, S::lanes, S::packs, S::threads, false>), grid, dim3(S::threads), 0, stream, a);
+        hipLaunchKernelGGL((norm_rows_kernel<T, S::lanes, S::packs, S::threads, RELU, DROP>), grid, dim3(S::threads), 0, stream, a);
         return check_launch("layer_norm");
     });
 }
@@ -186,12 +182,12 @@ extern "C" int cgnn_layer_norm(int64_t rows, int64_t F, int dtype, int param_dty
         a.weight = {weight, param_dtype != dtype};
         a.bias = {bias, param_dtype != dtype};
         a.eps = eps;
-        a.relu = relu;
         a.drop = drop_of(drop, F);
         a.out = static_cast<T *>(out);
         a.stats = stats;
         a.rows = rows;
         a.F = F;
-        return norm_typed<T>(a, a.drop.kept < kAllKept, stream);
+        if (a.drop.kept < kAllKept) return relu ? norm_launch<T, true, true>(a, stream) : norm_launch<T, false, true>(a, stream);
+        return relu ? norm_launch<T, true, false>(a, stream) : norm_launch<T, false, false>(a, stream);
     });
 }

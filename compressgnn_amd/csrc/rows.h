@@ -68,6 +68,12 @@ inline Drop drop_of(const cgnn_drop *d, int64_t F) {
 
 #define CGNN_REQUIRE_DROP(op, d) CGNN_REQUIRE((d)->kept >= 0 && (d)->kept <= (int32_t)kAllKept, op ": kept must lie in [0, 65536]")
 
+// By value: a choice between elements of an array would be one between addresses, and put the array into memory.
+template <typename T>
+__device__ __forceinline__ T either(bool first, T a, T b) {
+    return first ? a : b;
+}
+
 // Eight draws of 16 bits, two a word, the low half first.
 struct Draws {
     uint32_t word[4];
@@ -78,9 +84,11 @@ struct Draws {
     // The N that begin at element j of a row come to the front (N divides j).
     template <int N>
     __device__ __forceinline__ void from(int j) {
-        const uint32_t w0 = word[0], w1 = word[1], w2 = word[2], w3 = word[3];
-        if constexpr (N <= 4) word[0] = j & 4 ? w2 : w0, word[1] = j & 4 ? w3 : w1;
-        if constexpr (N == 2) word[0] = j & 2 ? word[1] : word[0];
+        if constexpr (N <= 4) {
+            word[0] = either(j & 4, word[2], word[0]);
+            word[1] = either(j & 4, word[3], word[1]);
+        }
+        if constexpr (N == 2) word[0] = either(j & 2, word[1], word[0]);
     }
 };
 
@@ -103,7 +111,10 @@ __device__ __forceinline__ Draws draw(uint64_t seed, uint64_t offset, uint64_t b
 
 __device__ __forceinline__ uint64_t drop_offset(const Drop &d) { return d.offset + (d.counter ? (uint64_t)*d.counter : 0); }
 
-// ------------------------------------------------------------------------- reading ----
+// --------------------------------------------------------------- reading and writing ----
+
+template <typename T, int N>
+using vec = T __attribute__((ext_vector_type(N)));
 
 // N elements at any element's address: loads and stores of 16 bytes where they make that many.  The memory of gfx950 takes them
 // at addresses that are no multiple of 16.
@@ -125,6 +136,68 @@ __device__ __forceinline__ Pack<T, N> load_pack(const T *row, int64_t j, int64_t
     return p;
 }
 
+// 16 bytes as they are: held this way, and not as elements, the words of a load in flight are not touched before they are used.
+typedef uint32_t words_t __attribute__((ext_vector_type(4), aligned(2), may_alias));
+
+// N elements (16 bytes) from `at` on of `extent` >= N elements: one load without a branch, so that nothing waits for it before its
+// values are used.  It may run into the next row (the caller has to leave what it finds there); where it would leave the matrix it reads
+// the last N elements instead, and `settled` gets the ones asked for once they are used.
+template <typename T>
+__device__ __forceinline__ words_t ask_within(const T *matrix, int64_t at, int64_t extent) {
+    constexpr int N = 16 / (int)sizeof(T);
+    return *reinterpret_cast<const words_t *>(matrix + (at < extent - N ? at : extent - N));
+}
+
+// Waits for what was asked for, here: loads and stores are counted together and in order, and a wait behind a store that not every
+// lane makes has to wait for that store too.  Ahead of a row's stores this waits for the next row's loads and the last
+// row's stores only, both asked for a row's work ago.  The same ahead of the loop, whose first waits would else be in every round.
+template <int K>
+__device__ __forceinline__ void arrived(words_t (&asked)[K]) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) asm volatile("" : "+v"(asked[k]));
+}
+
+template <typename C, int K, int N>
+__device__ __forceinline__ void arrived(C (&asked)[K][N]) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < N; ++i) asm volatile("" : "+v"(asked[k][i]));
+}
+
+template <typename T>
+__device__ __forceinline__ void arrived(T &asked) {
+    if constexpr (sizeof(T) == 2) {
+        uint32_t word = __builtin_bit_cast(uint16_t, asked);
+        asm volatile("" : "+v"(word));
+        asked = __builtin_bit_cast(T, (uint16_t)word);
+    } else {
+        asm volatile("" : "+v"(asked));
+    }
+}
+
+template <typename T, int N = 16 / (int)sizeof(T)>
+__device__ __forceinline__ Pack<T, N> settled(words_t asked, const T *matrix, int64_t at, int64_t extent) {
+    Pack<T, N> p = __builtin_bit_cast(Pack<T, N>, asked);
+    if (at > extent - N)
+#pragma unroll
+        for (int i = 0; i < N; ++i) p.v[i] = matrix[at + i < extent ? at + i : extent - 1];
+    return p;
+}
+
+// The same at once, for any extent.
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_within(const T *matrix, int64_t at, int64_t extent) {
+    Pack<T, N> p;
+    if (at + N <= extent) {
+        p = *reinterpret_cast<const Pack<T, N> *>(matrix + at);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) p.v[i] = matrix[at + i < extent ? at + i : extent - 1];
+    }
+    return p;
+}
+
 template <typename T, int N>
 __device__ __forceinline__ void store_pack(T *row, int64_t j, int64_t F, const Pack<T, N> &p) {
     if (j + N <= F) {
@@ -134,6 +207,49 @@ __device__ __forceinline__ void store_pack(T *row, int64_t j, int64_t F, const P
         for (int i = 0; i < N; ++i)
             if (j + i < F) row[j + i] = p.v[i];
     }
+}
+
+// store_pack for a column j that is a multiple of N: what is left of the row has the same length, F % N, in every row, and goes out in
+// at most three pieces.
+template <typename T, int N>
+__device__ __forceinline__ void store_columns(T *row, int j, int F, const Pack<T, N> &p) {
+    if (j + N <= F) {
+        *reinterpret_cast<Pack<T, N> *>(row + j) = p;
+    } else if (j < F) {
+        const int rest = F % N;
+        T *to = row + j;
+        if constexpr (N == 8) {
+            const bool four = rest & 4, two = rest & 2;
+            if (four) *reinterpret_cast<Pack<T, 4> *>(to) = Pack<T, 4>{{p.v[0], p.v[1], p.v[2], p.v[3]}};
+            to += rest & 4;
+            const T a = either(four, p.v[4], p.v[0]), b = either(four, p.v[5], p.v[1]), c = either(four, p.v[6], p.v[2]);
+            if (two) *reinterpret_cast<Pack<T, 2> *>(to) = Pack<T, 2>{{a, b}};
+            if (rest & 1) to[rest & 2] = either(two, c, a);
+        } else if constexpr (N == 4) {
+            if (rest & 2) *reinterpret_cast<Pack<T, 2> *>(to) = Pack<T, 2>{{p.v[0], p.v[1]}};
+            if (rest & 1) to[rest & 2] = either(rest & 2, p.v[2], p.v[0]);
+        } else {
+            to[0] = p.v[0];
+        }
+    }
+}
+
+// Values rounded to the type of a row, two a step where the type has such a step.
+template <typename T, int N, typename C>
+__device__ __forceinline__ Pack<T, N> rounded(const C (&v)[N]) {
+    Pack<T, N> p;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const vec<T, 2> two = __builtin_convertvector((vec<float, 2>{v[i], v[i + 1]}), vec<T, 2>);
+            p.v[i] = two[0];
+            p.v[i + 1] = two[1];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) p.v[i] = (T)v[i];
+    }
+    return p;
 }
 
 // --------------------------------------------------------------------- sums of lanes ----
@@ -256,9 +372,21 @@ template <typename T>
 struct Params {
     const void *data;
     bool wide;
-    __device__ __forceinline__ compute_t<T> at(int64_t j, compute_t<T> otherwise) const {
-        if (data == nullptr) return otherwise;
-        return wide ? (compute_t<T>)static_cast<const float *>(data)[j] : (compute_t<T>)static_cast<const T *>(data)[j];
+    // Columns j ... j + N - 1; what lies behind F is not used by the caller.
+    template <int N>
+    __device__ __forceinline__ void read(int64_t j, int64_t F, compute_t<T> otherwise, compute_t<T> (&v)[N]) const {
+        if (data == nullptr || j >= F) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = otherwise;
+        } else if (wide) {
+            const auto p = load_within<float, N>(static_cast<const float *>(data), j, F);
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = (compute_t<T>)p.v[i];
+        } else {
+            const auto p = load_within<T, N>(static_cast<const T *>(data), j, F);
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = (compute_t<T>)p.v[i];
+        }
     }
 };
 
@@ -282,51 +410,66 @@ struct NormArgs {
     int64_t rows, F;
 };
 
-// What the ReLU sees of elements i = 0 ... N - 1: v = h w + b with h = (x - m) r, h in `h` too.  Forward pass and
-// gradient call this with the same numbers, and the side of zero that v is on is that of its value in 64 bits:
-// h is rounded once and h w + b once, so v is less than 2^-24 (|b| + 2 |v|) off and its sign is certain where |v| > 2^-21 |b|;
-// the few elements in between (one of a million, and those that are 0) are computed again.  A float decision alone would let
-// a sum of a million elements differ by a whole gradient now and then.
-template <int N, typename T, typename C>
-__device__ __forceinline__ void normalised(const T (&x)[N], double mean, double rstd, const C (&w)[N], const C (&b)[N], bool relu,
-                                           C (&h)[N], C (&v)[N]) {
+// Mean and reciprocal deviation of a row as its elements meet them.  In float the mean is two numbers, the nearest float and what is left
+// of it, so that a difference to it has one rounding and no offset costs bits.
+template <typename C>
+struct Centre {
+    double mean, rstd;
+    C near, scale, rest;
+    __device__ __forceinline__ Centre(double m, double r) : mean(m), rstd(r), near((C)m), scale((C)r), rest(-(C)(m - (double)near) * scale) {}
+    __device__ __forceinline__ C of(C x) const { return fused(x - near, scale, rest); }
+};
+
+// h = (x - m) r and v = h w + b of N elements.  Forward pass and gradient call this with the same numbers, and with RELU the
+// side of zero that v is on is that of its value in 64 bits: h takes three roundings and v one more, so v is less than
+// 2^-22 (|b| + |v|) off and its sign is certain where |v| > 2^-21 |b|; the few packs that come closer (one of 100,000) are
+// computed again.  A float decision alone would let a sum over a million elements be a whole gradient off now and then.
+template <bool RELU, int N, typename T, typename C>
+__device__ __forceinline__ void normalised(const T (&x)[N], const Centre<C> &centre, const C (&w)[N], const C (&b)[N], C (&h)[N], C (&v)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        h[i] = (C)(((double)x[i] - mean) * rstd);
+        h[i] = centre.of((C)x[i]);
         v[i] = fused(h[i], w[i], b[i]);
     }
-    if constexpr (sizeof(C) == 4) {
-        if (!relu) return;
-        bool unsure = false;
+    if constexpr (RELU && sizeof(C) == 4) {
+        float nearest = __builtin_fabsf(v[0]), largest = __builtin_fabsf(b[0]);
 #pragma unroll
-        for (int i = 0; i < N; ++i) unsure = unsure || __builtin_fabsf(v[i]) <= __builtin_fabsf(b[i]) * 0x1p-21f;
-        if (unsure)
+        for (int i = 1; i < N; ++i) {
+            nearest = __builtin_fminf(nearest, __builtin_fabsf(v[i]));
+            largest = __builtin_fmaxf(largest, __builtin_fabsf(b[i]));
+        }
+        if (nearest <= largest * 0x1p-21f) {
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (__builtin_fabsf(v[i]) <= __builtin_fabsf(b[i]) * 0x1p-21f) {
-                    float weight = w[i], bias = b[i];
-                    asm volatile("" : "+v"(weight), "+v"(bias));  // widened here: not ahead of the rows, in registers of its own
-                    v[i] = (C)__builtin_fma(((double)x[i] - mean) * rstd, (double)weight, (double)bias);
-                }
+            for (int i = 0; i < N; ++i) {
+                float weight = w[i], bias = b[i];
+                asm volatile("" : "+v"(weight), "+v"(bias));  // widened here: not ahead of the rows, in registers of its own
+                const double exact = __builtin_fma(((double)x[i] - centre.mean) * centre.rstd, (double)weight, (double)bias);
+                if (__builtin_fabsf(v[i]) <= largest * 0x1p-21f) v[i] = (C)exact;
+            }
+        }
     }
 }
 
-constexpr int64_t kMostPacks = 2048;  // of 16 bytes: longer rows do not fit the registers of a workgroup
-
-// How a row is spread: packs of 16 bytes over `lanes` lanes, `packs` on each; a workgroup has `threads`.  0 lanes:
-// more packs than most_packs.
+// How a row is spread: packs of 16 bytes over `lanes` lanes, `packs` on each; a workgroup has `threads`.  0 lanes: too long for
+// registers.  A lane has eight columns in a pack of a 16-bit row, with parameters, values and sums in float: two packs a lane are
+// beyond the 128 registers that a workgroup of 1,024 leaves it.
 struct RowShape {
     int lanes, packs, threads;
 };
 
-inline RowShape row_shape(int64_t F, size_t element, int64_t most_packs) {
+constexpr int64_t most_packs(size_t element) { return element == 2 ? 1024 : 2048; }
+
+inline RowShape row_shape(int64_t F, size_t element) {
     const int64_t packs = ceil_div(F, 16 / (int64_t)element);
-    if (packs > most_packs) return {0, 0, 1024};
+    if (packs > most_packs(element)) return {0, 0, 1024};
     if (packs <= 64) return {pow2_ceil(packs), 1, kBlock};
     if (packs <= 128) return {64, 2, kBlock};
     if (packs <= 512) return {256, packs <= 256 ? 1 : 2, 256};
     return {1024, packs <= 1024 ? 1 : 2, 1024};
 }
+
+// Whether a matrix has elements enough for one load of 16 bytes: the kernels that hold rows in registers make no smaller ones.
+inline bool loads_whole(int64_t rows, int64_t F, int64_t ld, size_t element) { return ((rows - 1) * ld + F) * (int64_t)element >= 16; }
 
 template <int LANES, int PACKS, int THREADS>
 struct ShapeTag {
@@ -334,7 +477,7 @@ struct ShapeTag {
 };
 
 // Calls `run` with the tag of a shape of at least one lane.
-template <typename F>
+template <typename T, typename F>
 int with_row_shape(const RowShape &s, F &&run) {
     switch (s.lanes) {
         case 1: return run(ShapeTag<1, 1, kBlock>());
@@ -345,7 +488,10 @@ int with_row_shape(const RowShape &s, F &&run) {
         case 32: return run(ShapeTag<32, 1, kBlock>());
         case 64: return s.packs == 1 ? run(ShapeTag<64, 1, kBlock>()) : run(ShapeTag<64, 2, kBlock>());
         case 256: return s.packs == 1 ? run(ShapeTag<256, 1, 256>()) : run(ShapeTag<256, 2, 256>());
-        default: return s.packs == 1 ? run(ShapeTag<1024, 1, 1024>()) : run(ShapeTag<1024, 2, 1024>());
+        default:
+            if constexpr (sizeof(T) > 2)
+                if (s.packs == 2) return run(ShapeTag<1024, 2, 1024>());
+            return run(ShapeTag<1024, 1, 1024>());
     }
 }
 
