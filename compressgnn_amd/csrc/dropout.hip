@@ -14,9 +14,11 @@ __global__ __launch_bounds__(kBlock) void dropout_kernel(const T *x, int64_t ldx
         const int64_t r = n / drop.blocks, j = (n - r * drop.blocks) * kDrawn;
         const Draws drawn = draw(drop.seed, offset, (uint64_t)n);
         const auto p = load_pack<T, kDrawn>(x + r * ldx, j, F);
-        Pack<T, kDrawn> y;
+        C v[kDrawn];
 #pragma unroll
-        for (int i = 0; i < kDrawn; ++i) y.v[i] = drawn.keeps(i, drop.kept) ? (T)((C)p.v[i] * (C)drop.scale) : T(0);
+        for (int i = 0; i < kDrawn; ++i) v[i] = (C)p.v[i] * (C)drop.scale;
+        auto y = rounded<T, kDrawn>(v);
+        if (drop.kept < kAllKept) y = masked<T, kDrawn>(y, drawn, drop.kept);
         store_pack<T, kDrawn>(out + r * F, j, F, y);
     }
 }

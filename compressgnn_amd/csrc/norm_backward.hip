@@ -11,15 +11,13 @@ namespace {
 constexpr int kLongRows = 64;   // rows longer than the registers: rows per part of the parameters' sums, at least
 constexpr int kLongParts = 512;
 constexpr int kLanes = 64;      // ... lanes side by side, kDrawn columns each
-constexpr int kChain = 512;     // other rows: as many of them at most are added up one after the other by a lane, in float
+constexpr int64_t kChain = 1024;  // other rows: as many of them at most are added up one after the other by a lane, in float
 
 int64_t long_rows(int64_t rows) { return std::max<int64_t>(kLongRows, ceil_div(rows, kLongParts)); }
 
-// Workgroups of norm_gradients_kernel, each of which leaves a part of the parameters' sums: as many as are resident, more
-// where the chains would get longer than kChain.
-int64_t row_parts(int64_t rows, const RowShape &s) {
-    const int64_t tiles = ceil_div(rows, s.threads / s.lanes);
-    return std::max(std::min<int64_t>(tiles, 256 * 1024 / s.threads), ceil_div(tiles, kChain));
+// Workgroups of norm_gradients_kernel, each of which leaves a part of the parameters' sums.
+int64_t row_parts(int64_t rows, const RowShape &s, size_t element) {
+    return std::max(row_workgroups(rows, s, element, true), ceil_div(rows, s.threads / s.lanes * kChain));
 }
 
 int64_t long_parts(int64_t rows) { return ceil_div(rows, long_rows(rows)); }
@@ -33,10 +31,11 @@ __global__ __launch_bounds__(THREADS) void norm_gradients_kernel(NormArgs<T> a) 
     constexpr int COLUMNS = LANES * K * N;  // that the lanes have room for
     __shared__ C scratch[LANES > kWave ? WAVES * 2 : WAVES * COLUMNS];
     const int lane = threadIdx.x % LANES, F = (int)a.F;
-    const int64_t step = (int64_t)gridDim.x * GROUPS;
     const int64_t extent_x = (a.rows - 1) * a.ldx + F, extent_g = (a.rows - 1) * a.ldg + F;
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
-    const C inverse_F = C(1) / (C)F;
+    // the dropout's scale is a factor of all sums and of dx: taken where those are done
+    const C inverse_F = C(1) / (C)F, dropped = DROP ? (C)a.drop.scale : C(1);
+    const int64_t step = (int64_t)gridDim.x * GROUPS;
     int64_t r = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LANES;
 
     words_t next_x[K], next_g[K];
@@ -77,20 +76,19 @@ __global__ __launch_bounds__(THREADS) void norm_gradients_kernel(NormArgs<T> a) 
         for (int k = 0; k < K; ++k) {
             const int j = (lane + k * LANES) * N, from = j < F ? j : 0;
             const auto x = settled<T>(next_x[k], a.x, r * a.ldx + from, extent_x);
-            const auto d = settled<T>(next_g[k], a.grad, r * a.ldg + from, extent_g);
+            auto d = settled<T>(next_g[k], a.grad, r * a.ldg + from, extent_g);
             C v[N];
             normalised<RELU, N>(x.v, centre, w[k], b[k], h[k], v);
             Draws drawn;
             if constexpr (DROP) {
                 drawn = draw(a.drop.seed, offset, (uint64_t)(r * a.drop.blocks + j / kDrawn));
                 drawn.from<N>(j);
+                d = masked<T, N>(d, drawn, a.drop.kept);
             }
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                C c = (C)d.v[i];
-                if constexpr (DROP) c = drawn.keeps(i, a.drop.kept) ? c * (C)a.drop.scale : C(0);
-                if constexpr (RELU) c = v[i] <= 0 ? C(0) : c;
-                g[k][i] = c;
+                g[k][i] = (C)d.v[i];
+                if constexpr (RELU) g[k][i] = v[i] <= 0 ? C(0) : g[k][i];
             }
             if (j + N > F)  // behind the row's end lies what the next one holds
 #pragma unroll
@@ -110,12 +108,12 @@ __global__ __launch_bounds__(THREADS) void norm_gradients_kernel(NormArgs<T> a) 
             }
         if (a.dx) {
             row_sums<LANES, THREADS>(sum, product, scratch);
-            const C c1 = sum * inverse_F, c2 = product * inverse_F;
+            const C c1 = sum * inverse_F, c2 = product * inverse_F, scale = centre.scale * dropped;
             Pack<T, N> dx[K];
 #pragma unroll
             for (int k = 0; k < K; ++k) {
 #pragma unroll
-                for (int i = 0; i < N; ++i) g[k][i] = centre.scale * (fused(-h[k][i], c2, g[k][i]) - c1);
+                for (int i = 0; i < N; ++i) g[k][i] = scale * (fused(-h[k][i], c2, g[k][i]) - c1);
                 dx[k] = rounded<T, N>(g[k]);
             }
             arrived(next_x);
@@ -136,7 +134,7 @@ __global__ __launch_bounds__(THREADS) void norm_gradients_kernel(NormArgs<T> a) 
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const int j = (lane + k * LANES) * N + i;
-                    if (j < F) columns[j] = acc[k][i];
+                    if (j < F) columns[j] = acc[k][i] * dropped;
                 }
         } else {
             __syncthreads();
@@ -152,7 +150,7 @@ __global__ __launch_bounds__(THREADS) void norm_gradients_kernel(NormArgs<T> a) 
                 C total = scratch[j];
 #pragma unroll
                 for (int wave = 1; wave < WAVES; ++wave) total += scratch[wave * COLUMNS + j];
-                columns[j] = total;
+                columns[j] = total * dropped;
             }
         }
     };
@@ -162,23 +160,21 @@ __global__ __launch_bounds__(THREADS) void norm_gradients_kernel(NormArgs<T> a) 
 
 // Eight elements of a row as the gradient sees them: h, and g as described above.
 template <typename T, bool RELU, bool DROP>
-__device__ __forceinline__ void masked(const NormArgs<T> &a, int64_t r, int64_t j, const Centre<compute_t<T>> &centre, uint64_t offset,
+__device__ __forceinline__ void read_masked(const NormArgs<T> &a, int64_t r, int64_t j, const Centre<compute_t<T>> &centre, uint64_t offset,
                                        compute_t<T> (&w)[kDrawn], compute_t<T> (&h)[kDrawn], compute_t<T> (&g)[kDrawn]) {
     using C = compute_t<T>;
     const auto x = load_pack<T, kDrawn>(a.x + r * a.ldx, j, a.F);
-    const auto d = load_pack<T, kDrawn>(a.grad + r * a.ldg, j, a.F);
+    auto d = load_pack<T, kDrawn>(a.grad + r * a.ldg, j, a.F);
     C b[kDrawn] = {}, v[kDrawn];
     a.weight.template read<kDrawn>(j, a.F, C(1), w);
     if constexpr (RELU) a.bias.template read<kDrawn>(j, a.F, C(0), b);
     normalised<RELU, kDrawn>(x.v, centre, w, b, h, v);
-    Draws drawn;
-    if constexpr (DROP) drawn = draw(a.drop.seed, offset, (uint64_t)(r * a.drop.blocks + j / kDrawn));
+    if constexpr (DROP) d = masked<T, kDrawn>(d, draw(a.drop.seed, offset, (uint64_t)(r * a.drop.blocks + j / kDrawn)), a.drop.kept);
 #pragma unroll
     for (int i = 0; i < kDrawn; ++i) {
-        C c = (C)d.v[i];
-        if constexpr (DROP) c = drawn.keeps(i, a.drop.kept) ? c * (C)a.drop.scale : C(0);
-        if constexpr (RELU) c = v[i] <= 0 ? C(0) : c;
-        g[i] = c;
+        g[i] = (C)d.v[i];
+        if constexpr (DROP) g[i] *= (C)a.drop.scale;
+        if constexpr (RELU) g[i] = v[i] <= 0 ? C(0) : g[i];
     }
 }
 
@@ -194,7 +190,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_dx_kernel(NormArgs<T> 
         const Centre<C> centre(a.stats[2 * r], a.stats[2 * r + 1]);
         C sum = 0, product = 0, w[kDrawn], h[kDrawn], g[kDrawn];
         for (int64_t j = (int64_t)threadIdx.x * kDrawn; j < a.F; j += (int64_t)kLongThreads * kDrawn) {
-            masked<T, RELU, DROP>(a, r, j, centre, offset, w, h, g);
+            read_masked<T, RELU, DROP>(a, r, j, centre, offset, w, h, g);
 #pragma unroll
             for (int i = 0; i < kDrawn; ++i) {
                 sum = fused(g[i], w[i], sum);
@@ -204,7 +200,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_dx_kernel(NormArgs<T> 
         row_sums<kLongThreads, kLongThreads>(sum, product, scratch);
         const C c1 = sum / (C)a.F, c2 = product / (C)a.F;
         for (int64_t j = (int64_t)threadIdx.x * kDrawn; j < a.F; j += (int64_t)kLongThreads * kDrawn) {
-            masked<T, RELU, DROP>(a, r, j, centre, offset, w, h, g);
+            read_masked<T, RELU, DROP>(a, r, j, centre, offset, w, h, g);
             C dx[kDrawn];
 #pragma unroll
             for (int i = 0; i < kDrawn; ++i) dx[i] = centre.scale * (fused(-h[i], c2, g[i] * w[i]) - c1);
@@ -226,7 +222,7 @@ __global__ __launch_bounds__(kBlock) void norm_long_parts_kernel(NormArgs<T> a, 
     if (j < a.F)
         for (int64_t r = (int64_t)blockIdx.x * part + group; r < last; r += kBlock / kLanes) {
             C w[kDrawn], h[kDrawn], g[kDrawn];
-            masked<T, RELU, DROP>(a, r, j, Centre<C>(a.stats[2 * r], a.stats[2 * r + 1]), offset, w, h, g);
+            read_masked<T, RELU, DROP>(a, r, j, Centre<C>(a.stats[2 * r], a.stats[2 * r + 1]), offset, w, h, g);
 #pragma unroll
             for (int i = 0; i < kDrawn; ++i) {
                 dw[i] = fused(g[i], h[i], dw[i]);
@@ -288,7 +284,7 @@ __global__ __launch_bounds__(kSumThreads) void norm_sum_parts_kernel(const C *pa
 template <typename T, bool RELU, bool DROP>
 int gradients_launch(const NormArgs<T> &a, const RowShape &shape, int64_t parts, hipStream_t stream) {
     if (shape.lanes)
-        return with_row_shape<T>(shape, [&](auto tag) {
+        return with_row_shape<T, true>(shape, [&](auto tag) {
             using S = decltype(tag);
             hipLaunchKernelGGL((norm_gradients_kernel<T, S::lanes, S::packs, S::threads, RELU, DROP>), dim3((unsigned)parts), dim3(S::threads),
                                0, stream, a);
@@ -308,9 +304,9 @@ int gradients_launch(const NormArgs<T> &a, const RowShape &shape, int64_t parts,
 template <typename T>
 int norm_backward_typed(NormArgs<T> a, bool drops, int param_dtype, void *dweight, void *dbias, hipStream_t stream) {
     using C = compute_t<T>;
-    RowShape shape = row_shape(a.F, sizeof(T));
+    RowShape shape = row_shape(a.F, sizeof(T), true);
     if (!loads_whole(a.rows, a.F, a.ldx, sizeof(T)) || !loads_whole(a.rows, a.F, a.ldg, sizeof(T))) shape.lanes = 0;
-    const int64_t parts = shape.lanes ? row_parts(a.rows, shape) : long_parts(a.rows);
+    const int64_t parts = shape.lanes ? row_parts(a.rows, shape, sizeof(T)) : long_parts(a.rows);
     const bool sums = dweight != nullptr || dbias != nullptr;
     if (!sums) a.partial = nullptr;
     const int rc = drops ? (a.relu ? gradients_launch<T, true, true>(a, shape, parts, stream) : gradients_launch<T, false, true>(a, shape, parts, stream))
@@ -333,8 +329,8 @@ using namespace cgnn;
 
 extern "C" size_t cgnn_layer_norm_backward_workspace_bytes(int64_t rows, int64_t F, int dtype) {
     if (rows <= 0 || F <= 0) return 0;
-    const RowShape shape = row_shape(F, row_type_bytes(dtype));
-    const int64_t parts = std::max(long_parts(rows), shape.lanes ? row_parts(rows, shape) : 0);  // rows that lie too close take the other way
+    const RowShape shape = row_shape(F, row_type_bytes(dtype), true);
+    const int64_t parts = std::max(long_parts(rows), shape.lanes ? row_parts(rows, shape, row_type_bytes(dtype)) : 0);  // rows that lie too close take the other way
     return (size_t)parts * 2 * (size_t)F * (dtype == CGNN_F64 ? 8 : 4);
 }
 

@@ -14,9 +14,10 @@ __global__ __launch_bounds__(THREADS) void norm_rows_kernel(NormArgs<T> a) {
     constexpr int N = 16 / (int)sizeof(T), GROUPS = THREADS / LANES;
     __shared__ double scratch[LANES > kWave ? THREADS / kWave * 2 : 1];
     const int lane = threadIdx.x % LANES, F = (int)a.F;
-    const int64_t step = (int64_t)gridDim.x * GROUPS, extent = (a.rows - 1) * a.ldx + F;
+    const int64_t extent = (a.rows - 1) * a.ldx + F;
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
     const double inverse_F = 1.0 / (double)F;
+    const int64_t step = (int64_t)gridDim.x * GROUPS;
     int64_t r = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LANES;
 
     words_t next[K];
@@ -81,10 +82,11 @@ __global__ __launch_bounds__(THREADS) void norm_rows_kernel(NormArgs<T> a) {
             }
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                if constexpr (RELU) v[i] = v[i] <= 0 ? C(0) : v[i];
-                if constexpr (DROP) v[i] = drawn.keeps(i, a.drop.kept) ? v[i] * (C)a.drop.scale : C(0);
+                if constexpr (RELU) v[i] = rectified(v[i]);
+                if constexpr (DROP) v[i] *= (C)a.drop.scale;
             }
             y[k] = rounded<T, N>(v);
+            if constexpr (DROP) y[k] = masked<T, N>(y[k], drawn, a.drop.kept);
         }
         arrived(next);
         arrived(next_first);
@@ -136,24 +138,26 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs<T> a) 
             if constexpr (DROP) drawn = draw(a.drop.seed, offset, (uint64_t)(r * a.drop.blocks + j / kDrawn));
 #pragma unroll
             for (int i = 0; i < kDrawn; ++i) {
-                if constexpr (RELU) v[i] = v[i] <= 0 ? C(0) : v[i];
-                if constexpr (DROP) v[i] = drawn.keeps(i, a.drop.kept) ? v[i] * (C)a.drop.scale : C(0);
+                if constexpr (RELU) v[i] = rectified(v[i]);
+                if constexpr (DROP) v[i] *= (C)a.drop.scale;
             }
-            store_pack<T, kDrawn>(out, j, a.F, rounded<T, kDrawn>(v));
+            auto y = rounded<T, kDrawn>(v);
+            if constexpr (DROP) y = masked<T, kDrawn>(y, drawn, a.drop.kept);
+            store_pack<T, kDrawn>(out, j, a.F, y);
         }
     }
 }
 
 template <typename T, bool RELU, bool DROP>
 int norm_launch(const NormArgs<T> &a, hipStream_t stream) {
-    const RowShape shape = row_shape(a.F, sizeof(T));
+    const RowShape shape = row_shape(a.F, sizeof(T), false);
     if (shape.lanes == 0 || !loads_whole(a.rows, a.F, a.ldx, sizeof(T))) {
         hipLaunchKernelGGL((norm_long_kernel<T, RELU, DROP>), dim3((unsigned)std::min<int64_t>(a.rows, 1024)), dim3(kLongThreads), 0, stream, a);
         return check_launch("layer_norm");
     }
-    return with_row_shape<T>(shape, [&](auto tag) {
+    return with_row_shape<T, false>(shape, [&](auto tag) {
         using S = decltype(tag);
-        const dim3 grid((unsigned)std::min<int64_t>(ceil_div(a.rows, S::threads / S::lanes), 256 * 2048 / S::threads));
+        const dim3 grid((unsigned)row_workgroups(a.rows, shape, sizeof(T), false));
         hipLaunchKernelGGL((norm_rows_kernel<T, S::lanes, S::packs, S::threads, RELU, DROP>), grid, dim3(S::threads), 0, stream, a);
         return check_launch("layer_norm");
     });

@@ -92,17 +92,18 @@ struct Draws {
     }
 };
 
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) { return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96); }
+
 __device__ __forceinline__ Draws draw(uint64_t seed, uint64_t offset, uint64_t block) {
     uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32), c2 = (uint32_t)offset, c3 = (uint32_t)(offset >> 32);
     uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
 #pragma unroll
     for (int round = 0; round < 10; ++round) {
         const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
-        const uint32_t n0 = (uint32_t)(b >> 32) ^ c1 ^ k0, n2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+        c0 = xor3((uint32_t)(b >> 32), c1, k0);
+        c2 = xor3((uint32_t)(a >> 32), c3, k1);
         c1 = (uint32_t)b;
         c3 = (uint32_t)a;
-        c0 = n0;
-        c2 = n2;
         k0 += 0x9E3779B9u;
         k1 += 0xBB67AE85u;
     }
@@ -234,17 +235,49 @@ __device__ __forceinline__ void store_columns(T *row, int j, int F, const Pack<T
     }
 }
 
+// p with the elements that are not kept zeroed (kept < 65536).  16-bit elements two a step: kept less the draw, not below zero, then at most one, times the
+// element's bits.
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> masked(const Pack<T, N> &p, const Draws &drawn, uint32_t kept) {
+    if constexpr (sizeof(T) == 2) {
+        struct Words {
+            uint32_t v[N / 2];
+        } words = __builtin_bit_cast(Words, p);
+        const uint32_t share = kept * 0x10001u;
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            uint32_t left;  // in assembly: the compiler makes two comparisons, two choices and a permutation of this
+            asm("v_pk_sub_u16 %0, %1, %2 clamp\n\tv_pk_min_u16 %0, %0, 1 op_sel_hi:[1,0]" : "=&v"(left) : "s"(share), "v"(drawn.word[i]));
+            asm("v_pk_mul_lo_u16 %0, %1, %2" : "=v"(words.v[i]) : "v"(words.v[i]), "v"(left));
+        }
+        return __builtin_bit_cast(Pack<T, N>, words);
+    } else {
+        Pack<T, N> out;
+#pragma unroll
+        for (int i = 0; i < N; ++i) out.v[i] = drawn.keeps(i, kept) ? p.v[i] : T(0);
+        return out;
+    }
+}
+
+// max(v, 0), and v where it is no number.
+template <typename C>
+__device__ __forceinline__ C rectified(C v) {
+    if constexpr (sizeof(C) == 4) return __builtin_elementwise_maximum(v, C(0));
+    return v <= 0 ? C(0) : v;
+}
+
 // Values rounded to the type of a row, two a step where the type has such a step.
 template <typename T, int N, typename C>
 __device__ __forceinline__ Pack<T, N> rounded(const C (&v)[N]) {
     Pack<T, N> p;
     if constexpr (sizeof(T) == 2) {
+        struct Words {
+            uint32_t v[N / 2];
+        } words;
 #pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const vec<T, 2> two = __builtin_convertvector((vec<float, 2>{v[i], v[i + 1]}), vec<T, 2>);
-            p.v[i] = two[0];
-            p.v[i + 1] = two[1];
-        }
+        for (int i = 0; i < N / 2; ++i)
+            words.v[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((vec<float, 2>{v[2 * i], v[2 * i + 1]}), vec<T, 2>));
+        p = __builtin_bit_cast(Pack<T, N>, words);
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) p.v[i] = (T)v[i];
@@ -451,21 +484,36 @@ __device__ __forceinline__ void normalised(const T (&x)[N], const Centre<C> &cen
 }
 
 // How a row is spread: packs of 16 bytes over `lanes` lanes, `packs` on each; a workgroup has `threads`.  0 lanes: too long for
-// registers.  A lane has eight columns in a pack of a 16-bit row, with parameters, values and sums in float: two packs a lane are
-// beyond the 128 registers that a workgroup of 1,024 leaves it.
+// registers.  The fewest places for the row's packs among powers of two with two or three packs a lane: several packs share the
+// additions across the lanes and what is computed once a row, and leave loads enough in flight for a few waves a SIMD.
+// Rows of 129 to 256 packs are one wave's, four packs a lane, in the forward pass (2,048 bfloat16 features, 43,945 rows: 75
+// against 80 us with a pack a lane of four waves); in the gradient, whose sums take registers too, four waves' with a pack a lane (124
+// against 144).  Of a 16-bit row a pack has eight columns, and a gradient's lane has registers for three packs, not four.
 struct RowShape {
     int lanes, packs, threads;
 };
 
-constexpr int64_t most_packs(size_t element) { return element == 2 ? 1024 : 2048; }
-
-inline RowShape row_shape(int64_t F, size_t element) {
+inline RowShape row_shape(int64_t F, size_t element, bool gradient) {
     const int64_t packs = ceil_div(F, 16 / (int64_t)element);
-    if (packs > most_packs(element)) return {0, 0, 1024};
-    if (packs <= 64) return {pow2_ceil(packs), 1, kBlock};
-    if (packs <= 128) return {64, 2, kBlock};
-    if (packs <= 512) return {256, packs <= 256 ? 1 : 2, 256};
-    return {1024, packs <= 1024 ? 1 : 2, 1024};
+    if (packs > (gradient && element == 2 ? 1536 : 2048)) return {0, 0, 0};
+    if (packs <= 3) return {1, (int)packs, kBlock};
+    if (packs <= 192) {
+        const int lanes = pow2_ceil(ceil_div(packs, 2));  // with two packs each; or half of them with three
+        if (lanes > kWave || packs <= 3 * (lanes / 2)) return {lanes / 2, 3, kBlock};
+        return {lanes, 2, kBlock};
+    }
+    if (packs <= 256) return gradient ? RowShape{256, 1, 256} : RowShape{64, 4, 256};
+    if (packs <= 768) return {256, packs <= 512 ? 2 : 3, 256};
+    return {512, packs <= 1024 ? 2 : packs <= 1536 ? 3 : 4, 512};
+}
+
+// Which rows the lane groups take: neighbours within a workgroup, and workgroup by workgroup, over and over, until all are
+// taken, so that the whole chip reads one stretch of memory at a time.  No more workgroups than are resident: a lane has its parameters in registers
+// and, in the gradient, its sums.
+inline int64_t row_workgroups(int64_t rows, const RowShape &s, size_t element, bool gradient) {
+    // waves a SIMD by the registers that a lane takes for its packs
+    const int64_t waves = s.packs == 1 ? 4 : s.packs > 2 ? 2 : !gradient ? 4 : s.lanes > kWave && element == 2 ? 2 : 3;
+    return std::min(ceil_div(rows, s.threads / s.lanes), 256 * 256 * waves / s.threads);
 }
 
 // Whether a matrix has elements enough for one load of 16 bytes: the kernels that hold rows in registers make no smaller ones.
@@ -477,21 +525,27 @@ struct ShapeTag {
 };
 
 // Calls `run` with the tag of a shape of at least one lane.
-template <typename T, typename F>
+template <typename T, bool GRADIENT, typename F>
 int with_row_shape(const RowShape &s, F &&run) {
     switch (s.lanes) {
-        case 1: return run(ShapeTag<1, 1, kBlock>());
-        case 2: return run(ShapeTag<2, 1, kBlock>());
-        case 4: return run(ShapeTag<4, 1, kBlock>());
-        case 8: return run(ShapeTag<8, 1, kBlock>());
-        case 16: return run(ShapeTag<16, 1, kBlock>());
-        case 32: return run(ShapeTag<32, 1, kBlock>());
-        case 64: return s.packs == 1 ? run(ShapeTag<64, 1, kBlock>()) : run(ShapeTag<64, 2, kBlock>());
-        case 256: return s.packs == 1 ? run(ShapeTag<256, 1, 256>()) : run(ShapeTag<256, 2, 256>());
+        case 1: return s.packs == 1 ? run(ShapeTag<1, 1, 256>()) : s.packs == 2 ? run(ShapeTag<1, 2, 256>()) : run(ShapeTag<1, 3, 256>());
+        case 2: return s.packs == 2 ? run(ShapeTag<2, 2, 256>()) : run(ShapeTag<2, 3, 256>());
+        case 4: return s.packs == 2 ? run(ShapeTag<4, 2, 256>()) : run(ShapeTag<4, 3, 256>());
+        case 8: return s.packs == 2 ? run(ShapeTag<8, 2, 256>()) : run(ShapeTag<8, 3, 256>());
+        case 16: return s.packs == 2 ? run(ShapeTag<16, 2, 256>()) : run(ShapeTag<16, 3, 256>());
+        case 32: return s.packs == 2 ? run(ShapeTag<32, 2, 256>()) : run(ShapeTag<32, 3, 256>());
+        case 64:
+            if constexpr (!GRADIENT)
+                if (s.packs == 4) return run(ShapeTag<64, 4, 256>());
+            return s.packs == 2 ? run(ShapeTag<64, 2, 256>()) : run(ShapeTag<64, 3, 256>());
+        case 256:
+            if constexpr (GRADIENT)
+                if (s.packs == 1) return run(ShapeTag<256, 1, 256>());
+            return s.packs == 2 ? run(ShapeTag<256, 2, 256>()) : run(ShapeTag<256, 3, 256>());
         default:
-            if constexpr (sizeof(T) > 2)
-                if (s.packs == 2) return run(ShapeTag<1024, 2, 1024>());
-            return run(ShapeTag<1024, 1, 1024>());
+            if constexpr (!GRADIENT || sizeof(T) > 2)
+                if (s.packs == 4) return run(ShapeTag<512, 4, 512>());
+            return s.packs == 2 ? run(ShapeTag<512, 2, 512>()) : run(ShapeTag<512, 3, 512>());
     }
 }
 
