@@ -72,6 +72,8 @@ __global__ __launch_bounds__(THREADS) void norm_gradients_kernel(NormArgs<T> a) 
         C h[K][N], g[K][N];
         const Centre<C> centre(next_mean, next_rstd);
         C sum = 0, product = 0;
+        Draws drawn[K];
+        if constexpr (DROP) draw_row<N, LANES>(a.drop.seed, offset, (uint64_t)(r * a.drop.blocks), lane, drawn);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int j = (lane + k * LANES) * N, from = j < F ? j : 0;
@@ -79,12 +81,7 @@ __global__ __launch_bounds__(THREADS) void norm_gradients_kernel(NormArgs<T> a) 
             auto d = settled<T>(next_g[k], a.grad, r * a.ldg + from, extent_g);
             C v[N];
             normalised<RELU, N>(x.v, centre, w[k], b[k], h[k], v);
-            Draws drawn;
-            if constexpr (DROP) {
-                drawn = draw(a.drop.seed, offset, (uint64_t)(r * a.drop.blocks + j / kDrawn));
-                drawn.from<N>(j);
-                d = masked<T, N>(d, drawn, a.drop.kept);
-            }
+            if constexpr (DROP) d = masked<T, N>(d, drawn[k], a.drop.kept);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 g[k][i] = (C)d.v[i];
@@ -121,7 +118,7 @@ __global__ __launch_bounds__(THREADS) void norm_gradients_kernel(NormArgs<T> a) 
             arrived(next_mean);
             arrived(next_rstd);
 #pragma unroll
-            for (int k = 0; k < K; ++k) store_columns<T, N>(a.dx + r * a.F, (lane + k * LANES) * N, F, dx[k]);
+            for (int k = 0; k < K; ++k) store_columns<T, N>(a.dx + r * a.F, (lane + k * LANES) * N, F, dx[k], a.streamed);
         }
     }
     if (a.partial == nullptr) return;
@@ -307,6 +304,7 @@ int norm_backward_typed(NormArgs<T> a, bool drops, int param_dtype, void *dweigh
     RowShape shape = row_shape(a.F, sizeof(T), true);
     if (!loads_whole(a.rows, a.F, a.ldx, sizeof(T)) || !loads_whole(a.rows, a.F, a.ldg, sizeof(T))) shape.lanes = 0;
     const int64_t parts = shape.lanes ? row_parts(a.rows, shape, sizeof(T)) : long_parts(a.rows);
+    if (shape.lanes) a.streamed = streams(a.rows, a.F * (int64_t)sizeof(T), shape.lanes * 16, 3);
     const bool sums = dweight != nullptr || dbias != nullptr;
     if (!sums) a.partial = nullptr;
     const int rc = drops ? (a.relu ? gradients_launch<T, true, true>(a, shape, parts, stream) : gradients_launch<T, false, true>(a, shape, parts, stream))

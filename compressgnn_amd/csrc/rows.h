@@ -110,9 +110,72 @@ __device__ __forceinline__ Draws draw(uint64_t seed, uint64_t offset, uint64_t b
     return Draws{{c0, c1, c2, c3}};
 }
 
+__device__ __forceinline__ uint32_t neighbours(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true); }
+__device__ __forceinline__ uint32_t across_pairs(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true); }
+
+// Packs of four: two lanes next to each other need half of the same eight draws.  Each makes those of one of two packs, the even
+// lane the first's, and they exchange the halves that the other needs.
+__device__ __forceinline__ void exchange(const Draws &own, bool odd, Draws &first, Draws &second) {
+    const uint32_t got0 = neighbours(either(odd, own.word[0], own.word[2])), got1 = neighbours(either(odd, own.word[1], own.word[3]));
+    first.word[0] = either(odd, got0, own.word[0]);
+    first.word[1] = either(odd, got1, own.word[1]);
+    second.word[0] = either(odd, own.word[2], got0);
+    second.word[1] = either(odd, own.word[3], got1);
+}
+
+// Packs of two: four lanes need a word each of the same eight draws.  Lane l of the four makes those of pack l of four, and the words
+// change places as rows and columns of a matrix do.
+__device__ __forceinline__ void exchange(Draws own, int lane, Draws (&packs)[4]) {
+    uint32_t(&w)[4] = own.word;
+    const bool odd = lane & 1, high = lane & 2;
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+        const uint32_t got = neighbours(either(odd, w[i], w[i + 1]));
+        w[i] = either(odd, got, w[i]);
+        w[i + 1] = either(odd, w[i + 1], got);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t got = across_pairs(either(high, w[i], w[i + 2]));
+        packs[i].word[0] = either(high, got, w[i]);
+        packs[i + 2].word[0] = either(high, w[i + 2], got);
+    }
+}
+
+// The draws of a lane's packs lane + k * LANES of a row whose numbers begin at `block`.
+template <int N, int LANES, int K>
+__device__ __forceinline__ void draw_row(uint64_t seed, uint64_t offset, uint64_t block, int lane, Draws (&drawn)[K]) {
+    if constexpr (N == 4 && LANES == 1) {  // a lane has both halves
+#pragma unroll
+        for (int k = 0; k < K; k += 2) {
+            drawn[k] = draw(seed, offset, block + k / 2);
+            if (k + 1 < K) {
+                drawn[k + 1].word[0] = drawn[k].word[2];
+                drawn[k + 1].word[1] = drawn[k].word[3];
+            }
+        }
+    } else {
+        constexpr int PAIRED = N == 4 ? K / 2 * 2 : 0;
+#pragma unroll
+        for (int k = 0; k < PAIRED; k += 2) {
+            const int pack = lane + k * LANES + (lane & 1) * LANES;
+            exchange(draw(seed, offset, block + pack / 2), lane & 1, drawn[k], drawn[k + 1]);
+        }
+#pragma unroll
+        for (int k = PAIRED; k < K; ++k) {
+            const int j = (lane + k * LANES) * N;
+            drawn[k] = draw(seed, offset, block + j / kDrawn);
+            drawn[k].template from<N>(j);
+        }
+    }
+}
+
 __device__ __forceinline__ uint64_t drop_offset(const Drop &d) { return d.offset + (d.counter ? (uint64_t)*d.counter : 0); }
 
 // --------------------------------------------------------------- reading and writing ----
+
+// 16 bytes as they are: held this way, and not as elements, the words of a load in flight are not touched before they are used.
+typedef uint32_t words_t __attribute__((ext_vector_type(4), aligned(2), may_alias));
 
 template <typename T, int N>
 using vec = T __attribute__((ext_vector_type(N)));
@@ -136,9 +199,6 @@ __device__ __forceinline__ Pack<T, N> load_pack(const T *row, int64_t j, int64_t
     }
     return p;
 }
-
-// 16 bytes as they are: held this way, and not as elements, the words of a load in flight are not touched before they are used.
-typedef uint32_t words_t __attribute__((ext_vector_type(4), aligned(2), may_alias));
 
 // N elements (16 bytes) from `at` on of `extent` >= N elements: one load without a branch, so that nothing waits for it before its
 // values are used.  It may run into the next row (the caller has to leave what it finds there); where it would leave the matrix it reads
@@ -210,14 +270,24 @@ __device__ __forceinline__ void store_pack(T *row, int64_t j, int64_t F, const P
     }
 }
 
+// 16 bytes, past the caches where they are not read again before they would be gone from there.  In assembly: of two stores that differ
+// in nothing else the compiler makes one, the plain one.
+template <typename T, int N>
+__device__ __forceinline__ void store_whole(T *to, const Pack<T, N> &p, bool streamed) {
+    if (streamed)
+        asm volatile("global_store_dwordx4 %0, %1, off nt" : : "v"(to), "v"(__builtin_bit_cast(words_t, p)) : "memory");
+    else
+        *reinterpret_cast<Pack<T, N> *>(to) = p;
+}
+
 // store_pack for a column j that is a multiple of N: what is left of the row has the same length, F % N, in every row, and goes out in
 // at most three pieces.
 template <typename T, int N>
-__device__ __forceinline__ void store_columns(T *row, int j, int F, const Pack<T, N> &p) {
+__device__ __forceinline__ void store_columns(T *row, int64_t j, int64_t F, const Pack<T, N> &p, bool streamed) {
     if (j + N <= F) {
-        *reinterpret_cast<Pack<T, N> *>(row + j) = p;
+        store_whole(row + j, p, streamed);
     } else if (j < F) {
-        const int rest = F % N;
+        const int rest = (int)(F % N);
         T *to = row + j;
         if constexpr (N == 8) {
             const bool four = rest & 4, two = rest & 2;
@@ -426,6 +496,12 @@ struct Params {
 __device__ __forceinline__ float fused(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 __device__ __forceinline__ double fused(double a, double b, double c) { return __builtin_fma(a, b, c); }
 
+// The rows of a lane group: every step-th one from its workgroup's first on, which lies `first` behind that of the workgroup before,
+// `rounds` of them at most.
+struct RowWalk {
+    int64_t first, step, rounds;
+};
+
 template <typename T>
 struct NormArgs {
     const T *x;
@@ -434,6 +510,8 @@ struct NormArgs {
     double eps;
     int relu;
     Drop drop;
+    RowWalk walk;
+    bool streamed;  // how the rows of the result are stored
     T *out;         // forward
     double *stats;  // [rows, 2]: mean and reciprocal deviation (written forward where wanted, read backward)
     const T *grad;  // backward
@@ -514,6 +592,13 @@ inline int64_t row_workgroups(int64_t rows, const RowShape &s, size_t element, b
     // waves a SIMD by the registers that a lane takes for its packs
     const int64_t waves = s.packs == 1 ? 4 : s.packs > 2 ? 2 : !gradient ? 4 : s.lanes > kWave && element == 2 ? 2 : 3;
     return std::min(ceil_div(rows, s.threads / s.lanes), 256 * 256 * waves / s.threads);
+}
+
+// Whether rows of a result are stored past the caches: where a pass moves more than the 256 MB of the last one hold, and the stores fill its
+// lines of 128 bytes (325,557 rows of 256 float16 features, forward: 56 us and 69 without; of 257, which fill none, 2,449,029 x 100
+// float32: 412 and 401; below that size there is nothing to gain, 325,557 x 64 float32: 27 and 27, and the reader behind to lose).
+inline bool streams(int64_t rows, int64_t row_bytes, int64_t store_bytes, int matrices) {
+    return rows * row_bytes * matrices > ((int64_t)256 << 20) && row_bytes % 128 == 0 && store_bytes >= 128;
 }
 
 // Whether a matrix has elements enough for one load of 16 bytes: the kernels that hold rows in registers make no smaller ones.
