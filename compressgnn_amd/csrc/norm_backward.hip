@@ -15,12 +15,29 @@ constexpr int64_t kChain = 1024;  // other rows: as many of them at most are add
 
 int64_t long_rows(int64_t rows) { return std::max<int64_t>(kLongRows, ceil_div(rows, kLongParts)); }
 
-// Workgroups of norm_gradients_kernel, each of which leaves a part of the parameters' sums.
+// Workgroups of norm_gradients_kernel, each of which leaves a part of the parameters' sums.  A part is two rows of floats: it is to stand for
+// sixteen rows or more (4,096 rows of 4,096 float16 features: 32 us with 256 parts, 35 with 512), if half the chip is not to be idle for that.
+// A few rows are one workgroup's, which then needs no second launch for the sums.
+constexpr int64_t kPartRows = 16, kFewestParts = 256, kAloneRounds = 4;
+
 int64_t row_parts(int64_t rows, const RowShape &s, size_t element) {
-    return std::max(row_workgroups(rows, s, element, true), ceil_div(rows, s.threads / s.lanes * kChain));
+    const int64_t groups = s.threads / s.lanes;
+    if (rows <= groups * kAloneRounds) return 1;
+    const int64_t most = std::min(row_workgroups(rows, s, element, true), std::max(kFewestParts, rows / kPartRows));
+    return std::max(most, ceil_div(rows, groups * kChain));
 }
 
 int64_t long_parts(int64_t rows) { return ceil_div(rows, long_rows(rows)); }
+
+int64_t parts_of(int64_t rows, const RowShape &s, size_t element) { return s.lanes ? row_parts(rows, s, element) : long_parts(rows); }
+
+// A sum of column j: to the part's place, or, where there is one part, to the result, of float or of the rows' type.
+template <typename T>
+__device__ __forceinline__ void leave_sum(compute_t<T> *part, void *whole, bool wide, int64_t j, compute_t<T> sum) {
+    if (part) part[j] = sum;
+    else if (whole && wide) static_cast<float *>(whole)[j] = (float)sum;
+    else if (whole) static_cast<T *>(whole)[j] = (T)sum;
+}
 
 // Rows that fit the registers of their lanes, as in the forward pass: x and the gradient are read once for dx and for
 // the parameters' sums, which every lane holds for its own columns until its rows are through.
@@ -121,17 +138,16 @@ __global__ __launch_bounds__(THREADS) void norm_gradients_kernel(NormArgs<T> a) 
             for (int k = 0; k < K; ++k) store_columns<T, N>(a.dx + r * a.F, (lane + k * LANES) * N, F, dx[k], a.streamed);
         }
     }
-    if (a.partial == nullptr) return;
+    if (a.partial == nullptr && a.dweight == nullptr && a.dbias == nullptr) return;
     // the lane groups of a wave, then its waves in their order
-    C *to = a.partial + (int64_t)blockIdx.x * 2 * a.F;
-    auto leave = [&](C(&acc)[K][N], C *columns) {
+    auto leave = [&](C(&acc)[K][N], C *part, void *whole) {
         if constexpr (LANES > kWave) {
 #pragma unroll
             for (int k = 0; k < K; ++k)
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const int j = (lane + k * LANES) * N + i;
-                    if (j < F) columns[j] = acc[k][i] * dropped;
+                    if (j < F) leave_sum<T>(part, whole, a.weight.wide, j, acc[k][i] * dropped);
                 }
         } else {
             __syncthreads();
@@ -147,12 +163,13 @@ __global__ __launch_bounds__(THREADS) void norm_gradients_kernel(NormArgs<T> a) 
                 C total = scratch[j];
 #pragma unroll
                 for (int wave = 1; wave < WAVES; ++wave) total += scratch[wave * COLUMNS + j];
-                columns[j] = total * dropped;
+                leave_sum<T>(part, whole, a.weight.wide, j, total * dropped);
             }
         }
     };
-    leave(dw, to);
-    leave(db, to + a.F);
+    C *part = a.partial ? a.partial + (int64_t)blockIdx.x * 2 * a.F : nullptr;
+    leave(dw, part, a.dweight);
+    leave(db, part ? part + a.F : nullptr, a.dbias);
 }
 
 // Eight elements of a row as the gradient sees them: h, and g as described above.
@@ -242,9 +259,9 @@ __global__ __launch_bounds__(kBlock) void norm_long_parts_kernel(NormArgs<T> a, 
                     w += sums[k][0][i][lane];
                     b += sums[k][1][i][lane];
                 }
-                C *to = a.partial + (int64_t)blockIdx.x * 2 * a.F + j + i;
-                to[0] = w;
-                to[a.F] = b;
+                C *to = a.partial ? a.partial + (int64_t)blockIdx.x * 2 * a.F : nullptr;
+                leave_sum<T>(to, a.dweight, a.weight.wide, j + i, w);
+                leave_sum<T>(to ? to + a.F : nullptr, a.dbias, a.weight.wide, j + i, b);
             }
 }
 
@@ -291,9 +308,9 @@ int gradients_launch(const NormArgs<T> &a, const RowShape &shape, int64_t parts,
         hipLaunchKernelGGL((norm_long_dx_kernel<T, RELU, DROP>), dim3((unsigned)std::min<int64_t>(a.rows, 1024)), dim3(kLongThreads), 0, stream, a);
         if (int rc = check_launch("layer_norm_backward")) return rc;
     }
-    if (a.partial) {
+    if (a.partial || a.dweight || a.dbias) {
         const dim3 grid((unsigned)parts, (unsigned)ceil_div(a.F, (int64_t)kLanes * kDrawn));
-        hipLaunchKernelGGL((norm_long_parts_kernel<T, RELU, DROP>), grid, dim3(kBlock), 0, stream, a, long_rows(a.rows));
+        hipLaunchKernelGGL((norm_long_parts_kernel<T, RELU, DROP>), grid, dim3(kBlock), 0, stream, a, ceil_div(a.rows, parts));
     }
     return check_launch("layer_norm_backward");
 }
@@ -302,14 +319,21 @@ template <typename T>
 int norm_backward_typed(NormArgs<T> a, bool drops, int param_dtype, void *dweight, void *dbias, hipStream_t stream) {
     using C = compute_t<T>;
     RowShape shape = row_shape(a.F, sizeof(T), true);
-    if (!loads_whole(a.rows, a.F, a.ldx, sizeof(T)) || !loads_whole(a.rows, a.F, a.ldg, sizeof(T))) shape.lanes = 0;
-    const int64_t parts = shape.lanes ? row_parts(a.rows, shape, sizeof(T)) : long_parts(a.rows);
+    int64_t parts = parts_of(a.rows, shape, sizeof(T));
+    if (!loads_whole(a.rows, a.F, a.ldx, sizeof(T)) || !loads_whole(a.rows, a.F, a.ldg, sizeof(T))) {
+        shape.lanes = 0;  // the way of long rows, with no more parts
+        parts = std::min(parts, long_parts(a.rows));
+    }
     if (shape.lanes) a.streamed = streams(a.rows, a.F * (int64_t)sizeof(T), shape.lanes * 16, 3);
-    const bool sums = dweight != nullptr || dbias != nullptr;
-    if (!sums) a.partial = nullptr;
+    const bool sums = dweight != nullptr || dbias != nullptr, alone = parts == 1;
+    if (!sums || alone) a.partial = nullptr;
+    if (alone) {
+        a.dweight = dweight;
+        a.dbias = dbias;
+    }
     const int rc = drops ? (a.relu ? gradients_launch<T, true, true>(a, shape, parts, stream) : gradients_launch<T, false, true>(a, shape, parts, stream))
                          : (a.relu ? gradients_launch<T, true, false>(a, shape, parts, stream) : gradients_launch<T, false, false>(a, shape, parts, stream));
-    if (rc != CGNN_OK || !sums) return rc;
+    if (rc != CGNN_OK || !sums || alone) return rc;
     const dim3 columns((unsigned)ceil_div(2 * a.F, kSumColumns));
     if (param_dtype == CGNN_F32)
         hipLaunchKernelGGL((norm_sum_parts_kernel<C, float>), columns, dim3(kSumThreads), 0, stream, a.partial, parts, a.F,
@@ -328,8 +352,8 @@ using namespace cgnn;
 extern "C" size_t cgnn_layer_norm_backward_workspace_bytes(int64_t rows, int64_t F, int dtype) {
     if (rows <= 0 || F <= 0) return 0;
     const RowShape shape = row_shape(F, row_type_bytes(dtype), true);
-    const int64_t parts = std::max(long_parts(rows), shape.lanes ? row_parts(rows, shape, row_type_bytes(dtype)) : 0);  // rows that lie too close take the other way
-    return (size_t)parts * 2 * (size_t)F * (dtype == CGNN_F64 ? 8 : 4);
+    const int64_t parts = parts_of(rows, shape, row_type_bytes(dtype));
+    return parts == 1 ? 0 : (size_t)parts * 2 * (size_t)F * (dtype == CGNN_F64 ? 8 : 4);
 }
 
 extern "C" int cgnn_layer_norm_backward(int64_t rows, int64_t F, int dtype, int param_dtype, const void *grad, int64_t ldg,
@@ -346,7 +370,7 @@ extern "C" int cgnn_layer_norm_backward(int64_t rows, int64_t F, int dtype, int 
         if (dx == nullptr && dweight == nullptr && dbias == nullptr) return (int)CGNN_OK;
         CGNN_REQUIRE(grad && x && stats, "cgnn_layer_norm_backward: null array");
         if ((dweight || dbias) &&
-            (workspace == nullptr || workspace_bytes < cgnn_layer_norm_backward_workspace_bytes(rows, F, dtype)))
+            (workspace_bytes < cgnn_layer_norm_backward_workspace_bytes(rows, F, dtype) || (workspace == nullptr && workspace_bytes)))
             return fail(CGNN_EWORKSPACE, "cgnn_layer_norm_backward: workspace too small");
         NormArgs<T> a{};
         a.x = static_cast<const T *>(x);

@@ -518,6 +518,7 @@ struct NormArgs {
     int64_t ldg;
     T *dx;           // or NULL
     compute_t<T> *partial;  // [parts, 2, F]: sums of g * h and of g over a part of the rows
+    void *dweight, *dbias;  // where there is one part, which has no need of partial; parameters' type
     int64_t rows, F;
 };
 
@@ -566,14 +567,15 @@ __device__ __forceinline__ void normalised(const T (&x)[N], const Centre<C> &cen
 // additions across the lanes and what is computed once a row, and leave loads enough in flight for a few waves a SIMD.
 // Rows of 129 to 256 packs are one wave's, four packs a lane, in the forward pass (2,048 bfloat16 features, 43,945 rows: 75
 // against 80 us with a pack a lane of four waves); in the gradient, whose sums take registers too, four waves' with a pack a lane (124
-// against 144).  Of a 16-bit row a pack has eight columns, and a gradient's lane has registers for three packs, not four.
+// against 144).  Of a 16-bit row a pack has eight columns, and the lanes of
+// 512 have registers for two packs in the gradient, not four.
 struct RowShape {
     int lanes, packs, threads;
 };
 
 inline RowShape row_shape(int64_t F, size_t element, bool gradient) {
     const int64_t packs = ceil_div(F, 16 / (int64_t)element);
-    if (packs > (gradient && element == 2 ? 1536 : 2048)) return {0, 0, 0};
+    if (packs > (gradient && element == 2 ? 1024 : 2048)) return {0, 0, 0};
     if (packs <= 3) return {1, (int)packs, kBlock};
     if (packs <= 192) {
         const int lanes = pow2_ceil(ceil_div(packs, 2));  // with two packs each; or half of them with three
@@ -629,8 +631,8 @@ int with_row_shape(const RowShape &s, F &&run) {
             return s.packs == 2 ? run(ShapeTag<256, 2, 256>()) : run(ShapeTag<256, 3, 256>());
         default:
             if constexpr (!GRADIENT || sizeof(T) > 2)
-                if (s.packs == 4) return run(ShapeTag<512, 4, 512>());
-            return s.packs == 2 ? run(ShapeTag<512, 2, 512>()) : run(ShapeTag<512, 3, 512>());
+                if (s.packs > 2) return s.packs == 3 ? run(ShapeTag<512, 3, 512>()) : run(ShapeTag<512, 4, 512>());
+            return run(ShapeTag<512, 2, 512>());
     }
 }
 

@@ -129,8 +129,12 @@ def test_entry_points_check_before_they_touch_the_device():
         assert _gradients(**call) == EINVAL, call
     assert _gradients(dtype=9, param=9) == EUNSUPPORTED
     assert _gradients() == 0  # nothing wanted
-    need = abi.lib().cgnn_layer_norm_backward_workspace_bytes(abi.i64(4), abi.i64(8), 0)
-    assert _gradients(dw=16) == EWORKSPACE and _gradients(dw=16, ws=16, bytes=need - 1) == EWORKSPACE
+    for rows, width, dtype in ((5000, 8, 0), (5000, 8, 3), (300, 100000, 2)):
+        need = abi.lib().cgnn_layer_norm_backward_workspace_bytes(abi.i64(rows), abi.i64(width), dtype)
+        call = dict(rows=rows, F=width, dtype=dtype, param=dtype, ldx=width, ldg=width, dw=16)
+        assert need > 0
+        assert _gradients(**call) == EWORKSPACE and _gradients(**call, ws=16, bytes=need - 1) == EWORKSPACE
+        assert _gradients(**call, ws=0, bytes=need) == EWORKSPACE
     assert abi.lib().cgnn_layer_norm_backward_workspace_bytes(abi.i64(0), abi.i64(8), 0) == 0
     # the graph and cluster entry points still take two types only
     assert abi.lib().cgnn_lsh_hash(abi.i64(4), abi.i64(4), 2, 2, None, None, None, None, None) != 0
