@@ -94,7 +94,7 @@ __global__ __launch_bounds__(kBlock) void dropout_few_kernel(DropoutArgs<T> a) {
 template <typename T>
 int dropout_launch(DropoutArgs<T> a, hipStream_t stream) {
     constexpr int N = 16 / (int)sizeof(T), SHARE = kDrawn / N, PACKS = SHARE < 2 ? 2 : SHARE;
-    if (!loads_whole(a.rows, a.F, a.ldx, sizeof(T))) {
+    if (a.rows * a.F * (int64_t)sizeof(T) < 16) {
         hipLaunchKernelGGL((dropout_few_kernel<T>), dim3(1), dim3(kBlock), 0, stream, a);
         return check_launch("dropout");
     }
@@ -121,7 +121,7 @@ using namespace cgnn;
 
 extern "C" int cgnn_dropout(int64_t rows, int64_t F, int dtype, const void *x, int64_t ldx, const cgnn_drop *drop, void *out,
                             cgnn_stream_t stream) {
-    CGNN_REQUIRE(rows >= 0 && F >= 0 && ldx >= 0, "cgnn_dropout: bad size");
+    CGNN_REQUIRE(rows >= 0 && F >= 0 && (rows <= 1 || ldx >= F), "cgnn_dropout: bad size");
     CGNN_REQUIRE(drop, "cgnn_dropout: null drop");
     CGNN_REQUIRE_DROP("cgnn_dropout", drop);
     return with_row_type(dtype, "cgnn_dropout: dtype must be f32, f64, f16 or bf16", [&](auto tag) {

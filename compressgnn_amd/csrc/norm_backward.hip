@@ -10,7 +10,7 @@ namespace {
 
 constexpr int kLongRows = 64;   // rows longer than the registers: rows per part of the parameters' sums, at least
 constexpr int kLongParts = 512;
-constexpr int kLanes = 64;      // ... lanes side by side, kDrawn columns each
+constexpr int kLanes = 64;      // ... lanes side by side, a pack each
 constexpr int64_t kChain = 1024;  // other rows: as many of them at most are added up one after the other by a lane, in float
 
 int64_t long_rows(int64_t rows) { return std::max<int64_t>(kLongRows, ceil_div(rows, kLongParts)); }
@@ -172,97 +172,192 @@ __global__ __launch_bounds__(THREADS) void norm_gradients_kernel(NormArgs<T> a) 
     leave(db, part ? part + a.F : nullptr, a.dbias);
 }
 
-// Eight elements of a row as the gradient sees them: h, and g as described above.
-template <typename T, bool RELU, bool DROP>
-__device__ __forceinline__ void read_masked(const NormArgs<T> &a, int64_t r, int64_t j, const Centre<compute_t<T>> &centre, uint64_t offset,
-                                       compute_t<T> (&w)[kDrawn], compute_t<T> (&h)[kDrawn], compute_t<T> (&g)[kDrawn]) {
+// A pack of a row as the gradient sees it: h, and g as described above but for the dropout's scale; zeros behind the row's end.
+template <typename T, bool RELU, bool DROP, int N>
+__device__ __forceinline__ void taken(const NormArgs<T> &a, const Pack<T, N> &x, Pack<T, N> d, int64_t r, int64_t j, const Centre<compute_t<T>> &centre,
+                                      const compute_t<T> (&w)[N], const compute_t<T> (&b)[N], uint64_t offset, compute_t<T> (&h)[N],
+                                      compute_t<T> (&g)[N]) {
     using C = compute_t<T>;
-    const auto x = load_pack<T, kDrawn>(a.x + r * a.ldx, j, a.F);
-    auto d = load_pack<T, kDrawn>(a.grad + r * a.ldg, j, a.F);
-    C b[kDrawn] = {}, v[kDrawn];
-    a.weight.template read<kDrawn>(j, a.F, C(1), w);
-    if constexpr (RELU) a.bias.template read<kDrawn>(j, a.F, C(0), b);
-    normalised<RELU, kDrawn>(x.v, centre, w, b, h, v);
-    if constexpr (DROP) d = masked<T, kDrawn>(d, draw(a.drop.seed, offset, (uint64_t)(r * a.drop.blocks + j / kDrawn)), a.drop.kept);
+    C v[N];
+    normalised<RELU, N>(x.v, centre, w, b, h, v);
+    if constexpr (DROP) {
+        Draws drawn = draw(a.drop.seed, offset, (uint64_t)(r * a.drop.blocks + j / kDrawn));
+        drawn.from<N>((int)(j % kDrawn));
+        d = masked<T, N>(d, drawn, a.drop.kept);
+    }
 #pragma unroll
-    for (int i = 0; i < kDrawn; ++i) {
+    for (int i = 0; i < N; ++i) {
         g[i] = (C)d.v[i];
-        if constexpr (DROP) g[i] *= (C)a.drop.scale;
         if constexpr (RELU) g[i] = v[i] <= 0 ? C(0) : g[i];
+        if (j + i >= a.F) h[i] = g[i] = C(0);
     }
 }
-
-constexpr int kLongThreads = 1024;
 
 // dx of longer rows: a workgroup per row, which reads it twice.
 template <typename T, bool RELU, bool DROP>
 __global__ __launch_bounds__(kLongThreads) void norm_long_dx_kernel(NormArgs<T> a) {
     using C = compute_t<T>;
+    constexpr int N = 16 / (int)sizeof(T), PACKS = sizeof(T) == 2 ? 1 : 2;  // as many as the registers hold
+    constexpr int64_t kStride = (int64_t)kLongThreads * N;
     __shared__ C scratch[kLongThreads / kWave * 2];
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
+    const int64_t extent_x = (a.rows - 1) * a.ldx + a.F, extent_g = (a.rows - 1) * a.ldg + a.F;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const Centre<C> centre(a.stats[2 * r], a.stats[2 * r + 1]);
-        C sum = 0, product = 0, w[kDrawn], h[kDrawn], g[kDrawn];
-        for (int64_t j = (int64_t)threadIdx.x * kDrawn; j < a.F; j += (int64_t)kLongThreads * kDrawn) {
-            read_masked<T, RELU, DROP>(a, r, j, centre, offset, w, h, g);
+        C sum = 0, product = 0, w[PACKS][N], b[PACKS][N], h[N], g[N];
+        words_t asked_x[PACKS], asked_g[PACKS];
+        auto ask = [&](int64_t j0) {
 #pragma unroll
-            for (int i = 0; i < kDrawn; ++i) {
-                sum = fused(g[i], w[i], sum);
-                product = fused(g[i] * w[i], h[i], product);
+            for (int k = 0; k < PACKS; ++k) {
+                const int64_t j = std::min(j0 + k * kStride, a.F - 1);
+                asked_x[k] = ask_within<T>(a.x, r * a.ldx + j, extent_x);
+                asked_g[k] = ask_within<T>(a.grad, r * a.ldg + j, extent_g);
+            }
+#pragma unroll
+            for (int k = 0; k < PACKS; ++k) {
+                a.weight.template read<N>(j0 + k * kStride, a.F, C(1), w[k]);
+                if constexpr (RELU) a.bias.template read<N>(j0 + k * kStride, a.F, C(0), b[k]);
+                if constexpr (!RELU)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) b[k][i] = C(0);
+            }
+        };
+        auto take = [&](int64_t j0, int k) {
+            const int64_t j = std::min(j0 + k * kStride, a.F - 1);
+            taken<T, RELU, DROP, N>(a, settled<T>(asked_x[k], a.x, r * a.ldx + j, extent_x), settled<T>(asked_g[k], a.grad, r * a.ldg + j, extent_g), r,
+                                    j0 + k * kStride, centre, w[k], b[k], offset, h, g);
+        };
+        for (int64_t j0 = (int64_t)threadIdx.x * N; j0 < a.F; j0 += PACKS * kStride) {
+            ask(j0);
+#pragma unroll
+            for (int k = 0; k < PACKS; ++k) {
+                take(j0, k);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const C gw = g[i] * w[k][i];
+                    sum += gw;
+                    product = fused(gw, h[i], product);
+                }
             }
         }
         row_sums<kLongThreads, kLongThreads>(sum, product, scratch);
-        const C c1 = sum / (C)a.F, c2 = product / (C)a.F;
-        for (int64_t j = (int64_t)threadIdx.x * kDrawn; j < a.F; j += (int64_t)kLongThreads * kDrawn) {
-            read_masked<T, RELU, DROP>(a, r, j, centre, offset, w, h, g);
-            C dx[kDrawn];
+        const C c1 = sum / (C)a.F, c2 = product / (C)a.F, scale = centre.scale * (DROP ? (C)a.drop.scale : C(1));
+        for (int64_t j0 = (int64_t)threadIdx.x * N; j0 < a.F; j0 += PACKS * kStride) {
+            ask(j0);
 #pragma unroll
-            for (int i = 0; i < kDrawn; ++i) dx[i] = centre.scale * (fused(-h[i], c2, g[i] * w[i]) - c1);
-            store_pack<T, kDrawn>(a.dx + r * a.F, j, a.F, rounded<T, kDrawn>(dx));
+            for (int k = 0; k < PACKS; ++k) {
+                take(j0, k);
+                C dx[N];
+#pragma unroll
+                for (int i = 0; i < N; ++i) dx[i] = scale * (fused(-h[i], c2, g[i] * w[k][i]) - c1);
+                store_columns<T, N>(a.dx + r * a.F, j0 + k * kStride, a.F, rounded<T, N>(dx), false);
+            }
         }
     }
 }
 
-// Their dw and db: blockIdx.x names the part, `part` rows each, blockIdx.y the columns.
+// Their dw and db: blockIdx.x names the part, `part` rows each, blockIdx.y the columns.  A lane keeps its columns and goes down the rows.
 template <typename T, bool RELU, bool DROP>
 __global__ __launch_bounds__(kBlock) void norm_long_parts_kernel(NormArgs<T> a, int64_t part) {
     using C = compute_t<T>;
-    __shared__ C sums[kBlock / kLanes][2][kDrawn][kLanes];
+    constexpr int N = 16 / (int)sizeof(T), GROUPS = kBlock / kLanes;
+    __shared__ C sums[GROUPS][2][N][kLanes];
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
+    const int64_t extent_x = (a.rows - 1) * a.ldx + a.F, extent_g = (a.rows - 1) * a.ldg + a.F;
     const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-    const int64_t j = ((int64_t)blockIdx.y * kLanes + lane) * kDrawn;
+    const int64_t j = ((int64_t)blockIdx.y * kLanes + lane) * N, from = std::min(j, a.F - 1);
     const int64_t last = std::min(a.rows, (int64_t)(blockIdx.x + 1) * part);
-    C dw[kDrawn] = {}, db[kDrawn] = {};
-    if (j < a.F)
-        for (int64_t r = (int64_t)blockIdx.x * part + group; r < last; r += kBlock / kLanes) {
-            C w[kDrawn], h[kDrawn], g[kDrawn];
-            read_masked<T, RELU, DROP>(a, r, j, Centre<C>(a.stats[2 * r], a.stats[2 * r + 1]), offset, w, h, g);
+    int64_t r = (int64_t)blockIdx.x * part + group;
+    words_t next_x[1] = {}, next_g[1] = {};
+    double next_mean = 0, next_rstd = 0;
+    auto ask = [&](int64_t row) {
+        next_mean = a.stats[2 * row];
+        next_rstd = a.stats[2 * row + 1];
+        next_x[0] = ask_within<T>(a.x, row * a.ldx + from, extent_x);
+        next_g[0] = ask_within<T>(a.grad, row * a.ldg + from, extent_g);
+    };
+    if (r < last) ask(r);
+    C w[N], b[N] = {}, dw[N] = {}, db[N] = {};
+    a.weight.template read<N>(j, a.F, C(1), w);
+    if constexpr (RELU) a.bias.template read<N>(j, a.F, C(0), b);
+    for (; r < last; r += GROUPS) {
+        const Centre<C> centre(next_mean, next_rstd);
+        const auto x = settled<T>(next_x[0], a.x, r * a.ldx + from, extent_x);
+        const auto d = settled<T>(next_g[0], a.grad, r * a.ldg + from, extent_g);
+        ask(r + GROUPS < last ? r + GROUPS : r);
+        C h[N], g[N];
+        taken<T, RELU, DROP, N>(a, x, d, r, j, centre, w, b, offset, h, g);
 #pragma unroll
-            for (int i = 0; i < kDrawn; ++i) {
-                dw[i] = fused(g[i], h[i], dw[i]);
-                db[i] += g[i];
-            }
+        for (int i = 0; i < N; ++i) {
+            dw[i] = fused(g[i], h[i], dw[i]);
+            db[i] += g[i];
         }
+    }
 #pragma unroll
-    for (int i = 0; i < kDrawn; ++i) {
+    for (int i = 0; i < N; ++i) {
         sums[group][0][i][lane] = dw[i];
         sums[group][1][i][lane] = db[i];
     }
     __syncthreads();
     if (group == 0)
 #pragma unroll
-        for (int i = 0; i < kDrawn; ++i)
+        for (int i = 0; i < N; ++i)
             if (j + i < a.F) {
-                C w = 0, b = 0;
+                const C dropped = DROP ? (C)a.drop.scale : C(1);
+                C weight = 0, bias = 0;
 #pragma unroll
-                for (int k = 0; k < kBlock / kLanes; ++k) {
-                    w += sums[k][0][i][lane];
-                    b += sums[k][1][i][lane];
+                for (int k = 0; k < GROUPS; ++k) {
+                    weight += sums[k][0][i][lane];
+                    bias += sums[k][1][i][lane];
                 }
                 C *to = a.partial ? a.partial + (int64_t)blockIdx.x * 2 * a.F : nullptr;
-                leave_sum<T>(to, a.dweight, a.weight.wide, j + i, w);
-                leave_sum<T>(to ? to + a.F : nullptr, a.dbias, a.weight.wide, j + i, b);
+                leave_sum<T>(to, a.dweight, a.weight.wide, j + i, weight * dropped);
+                leave_sum<T>(to ? to + a.F : nullptr, a.dbias, a.weight.wide, j + i, bias * dropped);
             }
+}
+
+// Matrices of less than 16 bytes: a lane a row for dx, then a lane a column for the sums.
+template <typename T, bool RELU, bool DROP>
+__global__ __launch_bounds__(kWave) void norm_few_gradients_kernel(NormArgs<T> a) {
+    using C = compute_t<T>;
+    const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
+    auto one = [&](int64_t r, int64_t j, C &h, C &g, C &weight) {
+        C w[1], b[1] = {}, hh[1], v[1];
+        a.weight.template read<1>(j, a.F, C(1), w);
+        if constexpr (RELU) a.bias.template read<1>(j, a.F, C(0), b);
+        const T x[1] = {a.x[r * a.ldx + j]};
+        normalised<RELU, 1>(x, Centre<C>(a.stats[2 * r], a.stats[2 * r + 1]), w, b, hh, v);
+        h = hh[0];
+        weight = w[0];
+        g = (C)a.grad[r * a.ldg + j];
+        if constexpr (DROP) g = draw(a.drop.seed, offset, (uint64_t)r).keeps((int)j, a.drop.kept) ? g * (C)a.drop.scale : C(0);
+        if constexpr (RELU) g = v[0] <= 0 ? C(0) : g;
+    };
+    C h, g, w;
+    const int64_t lane = threadIdx.x;
+    if (a.dx && lane < a.rows) {
+        C sum = 0, product = 0;
+        for (int64_t j = 0; j < a.F; ++j) {
+            one(lane, j, h, g, w);
+            sum += g * w;
+            product = fused(g * w, h, product);
+        }
+        const C c1 = sum / (C)a.F, c2 = product / (C)a.F, scale = (C)a.stats[2 * lane + 1];
+        for (int64_t j = 0; j < a.F; ++j) {
+            one(lane, j, h, g, w);
+            a.dx[lane * a.F + j] = (T)(scale * (fused(-h, c2, g * w) - c1));
+        }
+    }
+    if (lane < a.F) {
+        C dw = 0, db = 0;
+        for (int64_t r = 0; r < a.rows; ++r) {
+            one(r, lane, h, g, w);
+            dw = fused(g, h, dw);
+            db += g;
+        }
+        leave_sum<T>((C *)nullptr, a.dweight, a.weight.wide, lane, dw);
+        leave_sum<T>((C *)nullptr, a.dbias, a.weight.wide, lane, db);
+    }
 }
 
 // The parts' sums, added up in 64 bits in an order that the number of parts fixes: column c < F of the weight's gradient, then
@@ -297,6 +392,10 @@ __global__ __launch_bounds__(kSumThreads) void norm_sum_parts_kernel(const C *pa
 
 template <typename T, bool RELU, bool DROP>
 int gradients_launch(const NormArgs<T> &a, const RowShape &shape, int64_t parts, hipStream_t stream) {
+    if (a.rows * a.F * (int64_t)sizeof(T) < 16) {
+        hipLaunchKernelGGL((norm_few_gradients_kernel<T, RELU, DROP>), dim3(1), dim3(kWave), 0, stream, a);
+        return check_launch("layer_norm_backward");
+    }
     if (shape.lanes)
         return with_row_shape<T, true>(shape, [&](auto tag) {
             using S = decltype(tag);
@@ -309,7 +408,7 @@ int gradients_launch(const NormArgs<T> &a, const RowShape &shape, int64_t parts,
         if (int rc = check_launch("layer_norm_backward")) return rc;
     }
     if (a.partial || a.dweight || a.dbias) {
-        const dim3 grid((unsigned)parts, (unsigned)ceil_div(a.F, (int64_t)kLanes * kDrawn));
+        const dim3 grid((unsigned)parts, (unsigned)ceil_div(a.F, (int64_t)kLanes * 16 / (int64_t)sizeof(T)));
         hipLaunchKernelGGL((norm_long_parts_kernel<T, RELU, DROP>), grid, dim3(kBlock), 0, stream, a, ceil_div(a.rows, parts));
     }
     return check_launch("layer_norm_backward");
@@ -318,12 +417,8 @@ int gradients_launch(const NormArgs<T> &a, const RowShape &shape, int64_t parts,
 template <typename T>
 int norm_backward_typed(NormArgs<T> a, bool drops, int param_dtype, void *dweight, void *dbias, hipStream_t stream) {
     using C = compute_t<T>;
-    RowShape shape = row_shape(a.F, sizeof(T), true);
-    int64_t parts = parts_of(a.rows, shape, sizeof(T));
-    if (!loads_whole(a.rows, a.F, a.ldx, sizeof(T)) || !loads_whole(a.rows, a.F, a.ldg, sizeof(T))) {
-        shape.lanes = 0;  // the way of long rows, with no more parts
-        parts = std::min(parts, long_parts(a.rows));
-    }
+    const RowShape shape = row_shape(a.F, sizeof(T), true);
+    const int64_t parts = parts_of(a.rows, shape, sizeof(T));
     if (shape.lanes) a.streamed = streams(a.rows, a.F * (int64_t)sizeof(T), shape.lanes * 16, 3);
     const bool sums = dweight != nullptr || dbias != nullptr, alone = parts == 1;
     if (!sums || alone) a.partial = nullptr;
@@ -360,7 +455,7 @@ extern "C" int cgnn_layer_norm_backward(int64_t rows, int64_t F, int dtype, int 
                                         const void *x, int64_t ldx, const double *stats, const void *weight, const void *bias,
                                         int relu, const cgnn_drop *drop, void *dx, void *dweight, void *dbias, void *workspace,
                                         size_t workspace_bytes, cgnn_stream_t stream) {
-    CGNN_REQUIRE(rows > 0 && F > 0 && ldx >= 0 && ldg >= 0, "cgnn_layer_norm_backward: bad size");
+    CGNN_REQUIRE(rows > 0 && F > 0 && (rows <= 1 || (ldx >= F && ldg >= F)), "cgnn_layer_norm_backward: bad size");
     CGNN_REQUIRE(F < ((int64_t)1 << 31) - 65536, "cgnn_layer_norm_backward: a row must be shorter than 2^31 elements");
     CGNN_REQUIRE(param_dtype == dtype || (param_dtype == CGNN_F32 && dtype != CGNN_F64),
                  "cgnn_layer_norm_backward: parameters have the type of the rows, or f32 for 16-bit rows");

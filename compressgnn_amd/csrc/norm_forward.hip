@@ -96,26 +96,37 @@ __global__ __launch_bounds__(THREADS) void norm_rows_kernel(NormArgs<T> a) {
     }
 }
 
-// Longer rows: a workgroup a row, which reads it twice.
-constexpr int kLongThreads = 1024;
-
+// Longer rows: a workgroup a row, which reads it twice, kLongPacks packs a lane at a time.
 template <typename T, bool RELU, bool DROP>
 __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs<T> a) {
     using C = compute_t<T>;
+    constexpr int N = 16 / (int)sizeof(T);
+    constexpr int64_t kStride = (int64_t)kLongThreads * N;
     __shared__ double scratch[kLongThreads / kWave * 2];
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
+    const int64_t extent = (a.rows - 1) * a.ldx + a.F;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const T *x = a.x + r * a.ldx;
-        T *out = a.out + r * a.F;
-        const double pivot = (double)x[0];
+        const int64_t at = r * a.ldx;
+        const T first = a.x[at];
+        const double pivot = (double)first;
         double sum = 0, squares = 0;
-        for (int64_t j = (int64_t)threadIdx.x * kDrawn; j < a.F; j += (int64_t)kLongThreads * kDrawn) {
-            const auto p = load_pack<T, kDrawn>(x, j, a.F);
+        words_t asked[kLongPacks];
+        auto ask = [&](int64_t j0) {
 #pragma unroll
-            for (int i = 0; i < kDrawn; ++i) {
-                const double d = j + i < a.F ? (double)p.v[i] - pivot : 0.0;
-                sum += d;
-                squares = __builtin_fma(d, d, squares);
+            for (int k = 0; k < kLongPacks; ++k) asked[k] = ask_within<T>(a.x, at + std::min(j0 + k * kStride, a.F - 1), extent);
+        };
+        for (int64_t j0 = (int64_t)threadIdx.x * N; j0 < a.F; j0 += kLongPacks * kStride) {
+            ask(j0);
+#pragma unroll
+            for (int k = 0; k < kLongPacks; ++k) {
+                const int64_t j = j0 + k * kStride;
+                const auto x = settled<T>(asked[k], a.x, at + std::min(j, a.F - 1), extent);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const double d = j + i < a.F ? (double)x.v[i] - pivot : 0.0;
+                    sum += d;
+                    squares = __builtin_fma(d, d, squares);
+                }
             }
         }
         row_sums<kLongThreads, kLongThreads>(sum, squares, scratch);
@@ -125,23 +136,66 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs<T> a) 
             a.stats[2 * r] = centre.mean;
             a.stats[2 * r + 1] = centre.rstd;
         }
-        for (int64_t j = (int64_t)threadIdx.x * kDrawn; j < a.F; j += (int64_t)kLongThreads * kDrawn) {
-            const auto p = load_pack<T, kDrawn>(x, j, a.F);
-            C w[kDrawn], b[kDrawn], h[kDrawn], v[kDrawn];
-            a.weight.template read<kDrawn>(j, a.F, C(1), w);
-            a.bias.template read<kDrawn>(j, a.F, C(0), b);
-            normalised<RELU, kDrawn>(p.v, centre, w, b, h, v);
-            Draws drawn;
-            if constexpr (DROP) drawn = draw(a.drop.seed, offset, (uint64_t)(r * a.drop.blocks + j / kDrawn));
+        for (int64_t j0 = (int64_t)threadIdx.x * N; j0 < a.F; j0 += kLongPacks * kStride) {
+            C w[kLongPacks][N], b[kLongPacks][N];
+            ask(j0);
 #pragma unroll
-            for (int i = 0; i < kDrawn; ++i) {
-                if constexpr (RELU) v[i] = rectified(v[i]);
-                if constexpr (DROP) v[i] *= (C)a.drop.scale;
+            for (int k = 0; k < kLongPacks; ++k) {
+                a.weight.template read<N>(j0 + k * kStride, a.F, C(1), w[k]);
+                a.bias.template read<N>(j0 + k * kStride, a.F, C(0), b[k]);
             }
-            auto y = rounded<T, kDrawn>(v);
-            if constexpr (DROP) y = masked<T, kDrawn>(y, drawn, a.drop.kept);
-            store_pack<T, kDrawn>(out, j, a.F, y);
+#pragma unroll
+            for (int k = 0; k < kLongPacks; ++k) {
+                const int64_t j = j0 + k * kStride;
+                const auto x = settled<T>(asked[k], a.x, at + std::min(j, a.F - 1), extent);
+                C h[N], v[N];
+                normalised<RELU, N>(x.v, centre, w[k], b[k], h, v);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    if constexpr (RELU) v[i] = rectified(v[i]);
+                    if constexpr (DROP) v[i] *= (C)a.drop.scale;
+                }
+                auto y = rounded<T, N>(v);
+                if constexpr (DROP) {
+                    Draws drawn = draw(a.drop.seed, offset, (uint64_t)(r * a.drop.blocks + j / kDrawn));
+                    drawn.from<N>((int)(j % kDrawn));
+                    y = masked<T, N>(y, drawn, a.drop.kept);
+                }
+                store_columns<T, N>(a.out + r * a.F, j, a.F, y, false);
+            }
         }
+    }
+}
+
+// Matrices of less than 16 bytes: a lane a row.
+template <typename T, bool RELU, bool DROP>
+__global__ __launch_bounds__(kWave) void norm_few_kernel(NormArgs<T> a) {
+    using C = compute_t<T>;
+    const int64_t r = threadIdx.x;
+    if (r >= a.rows) return;
+    const T *x = a.x + r * a.ldx;
+    double sum = 0, squares = 0;
+    for (int64_t j = 0; j < a.F; ++j) {
+        const double d = (double)x[j] - (double)x[0];
+        sum += d;
+        squares = __builtin_fma(d, d, squares);
+    }
+    const Moments m = moments((double)x[0], sum, squares, 1.0 / (double)a.F);
+    const Centre<C> centre(m.mean, reciprocal_root(m.variance + a.eps));
+    if (a.stats) {
+        a.stats[2 * r] = centre.mean;
+        a.stats[2 * r + 1] = centre.rstd;
+    }
+    const Draws drawn = DROP ? draw(a.drop.seed, drop_offset(a.drop), (uint64_t)r) : Draws{};  // F < 8: one call a row
+    for (int64_t j = 0; j < a.F; ++j) {
+        const T one[1] = {x[j]};
+        C w[1], b[1], h[1], v[1];
+        a.weight.template read<1>(j, a.F, C(1), w);
+        a.bias.template read<1>(j, a.F, C(0), b);
+        normalised<RELU, 1>(one, centre, w, b, h, v);
+        if constexpr (RELU) v[0] = rectified(v[0]);
+        if constexpr (DROP) v[0] = drawn.keeps((int)j, a.drop.kept) ? v[0] * (C)a.drop.scale : C(0);
+        a.out[r * a.F + j] = (T)v[0];
     }
 }
 
@@ -150,7 +204,11 @@ constexpr int64_t kLargeRounds = 8;
 template <typename T, bool RELU, bool DROP>
 int norm_launch(NormArgs<T> a, hipStream_t stream) {
     const RowShape shape = row_shape(a.F, sizeof(T), false);
-    if (shape.lanes == 0 || !loads_whole(a.rows, a.F, a.ldx, sizeof(T))) {
+    if (a.rows * a.F * (int64_t)sizeof(T) < 16) {
+        hipLaunchKernelGGL((norm_few_kernel<T, RELU, DROP>), dim3(1), dim3(kWave), 0, stream, a);
+        return check_launch("layer_norm");
+    }
+    if (shape.lanes == 0) {
         hipLaunchKernelGGL((norm_long_kernel<T, RELU, DROP>), dim3((unsigned)std::min<int64_t>(a.rows, 1024)), dim3(kLongThreads), 0, stream, a);
         return check_launch("layer_norm");
     }
@@ -181,7 +239,7 @@ using namespace cgnn;
 extern "C" int cgnn_layer_norm(int64_t rows, int64_t F, int dtype, int param_dtype, const void *x, int64_t ldx,
                                const void *weight, const void *bias, double eps, int relu, const cgnn_drop *drop, void *out,
                                double *stats, cgnn_stream_t stream) {
-    CGNN_REQUIRE(rows >= 0 && F >= 0 && ldx >= 0, "cgnn_layer_norm: bad size");
+    CGNN_REQUIRE(rows >= 0 && F >= 0 && (rows <= 1 || ldx >= F), "cgnn_layer_norm: bad size");
     CGNN_REQUIRE(eps >= 0, "cgnn_layer_norm: eps must not be negative");
     CGNN_REQUIRE(param_dtype == dtype || (param_dtype == CGNN_F32 && dtype != CGNN_F64),
                  "cgnn_layer_norm: parameters have the type of the rows, or f32 for 16-bit rows");

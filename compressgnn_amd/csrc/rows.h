@@ -475,7 +475,7 @@ template <typename T>
 struct Params {
     const void *data;
     bool wide;
-    // Columns j ... j + N - 1; what lies behind F is not used by the caller.
+    // Columns j ... j + N - 1; zeros behind F.
     template <int N>
     __device__ __forceinline__ void read(int64_t j, int64_t F, compute_t<T> otherwise, compute_t<T> (&v)[N]) const {
         if (data == nullptr || j >= F) {
@@ -490,6 +490,10 @@ struct Params {
 #pragma unroll
             for (int i = 0; i < N; ++i) v[i] = (compute_t<T>)p.v[i];
         }
+        if (j + N > F)
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (j + i >= F) v[i] = compute_t<T>(0);
     }
 };
 
@@ -603,8 +607,8 @@ inline bool streams(int64_t rows, int64_t row_bytes, int64_t store_bytes, int ma
     return rows * row_bytes * matrices > ((int64_t)256 << 20) && row_bytes % 128 == 0 && store_bytes >= 128;
 }
 
-// Whether a matrix has elements enough for one load of 16 bytes: the kernels that hold rows in registers make no smaller ones.
-inline bool loads_whole(int64_t rows, int64_t F, int64_t ld, size_t element) { return ((rows - 1) * ld + F) * (int64_t)element >= 16; }
+// The kernels of longer rows: a workgroup of the largest size a row, some loads of each lane in flight.
+constexpr int kLongThreads = 1024, kLongPacks = 3;
 
 template <int LANES, int PACKS, int THREADS>
 struct ShapeTag {

@@ -1653,7 +1653,7 @@ Rows rows_of(const char *op, const char *name, const Tensor &t) {
                 !t.defined() ? "undefined" : t.layout() == torch::kStrided ? seen(t) : c10::str(type, t.sizes(), " of layout ", t.layout()));
     const int64_t width = t.dim() ? t.size(-1) : 1;
     const Tensor plain = t.is_neg() ? t.resolve_neg() : t;
-    if (plain.dim() == 2 && (width <= 1 || plain.stride(1) == 1)) return {plain, plain.size(0), width, plain.stride(0)};
+    if (plain.dim() == 2 && (width <= 1 || plain.stride(1) == 1) && (plain.size(0) <= 1 || plain.stride(0) >= width)) return {plain, plain.size(0), width, plain.stride(0)};
     const Tensor dense = plain.contiguous();
     return {dense, width ? dense.numel() / width : 0, width, width};
 }

@@ -442,7 +442,7 @@ typedef struct cgnn_drop {
     int32_t kept;
 } cgnn_drop;
 
-/* out[i,j] = kept ? x[i,j] * 65536 / kept : 0; a dropped element is 0 whatever it holds.  x has rows ldx elements
+/* out[i,j] = kept ? x[i,j] * 65536 / kept : 0; a dropped element is 0 whatever it holds.  x has rows ldx >= F elements
  * apart, out is dense.  The gradient is the same call on the output's gradient. */
 int cgnn_dropout(int64_t rows, int64_t F, int dtype, const void *x, int64_t ldx, const cgnn_drop *drop, void *out,
                  cgnn_stream_t stream);

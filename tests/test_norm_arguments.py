@@ -114,7 +114,7 @@ def _kept(kept):
 
 def test_entry_points_check_before_they_touch_the_device():
     """Every call here is refused, or has nothing to do, on the host: no address in it is ever read."""
-    for call in (dict(rows=-1), dict(F=-1), dict(ldx=-1), dict(x=0), dict(out=0), dict(drop=_kept(-1)), dict(drop=_kept(65537))):
+    for call in (dict(rows=-1), dict(F=-1), dict(ldx=-1), dict(ldx=7), dict(x=0), dict(out=0), dict(drop=_kept(-1)), dict(drop=_kept(65537))):
         assert _norm(**call) == EINVAL and _dropout(**call) == EINVAL, call
     assert _dropout(drop=None) == EINVAL
     for eps in (-1e-9, float("nan")):
@@ -125,7 +125,7 @@ def test_entry_points_check_before_they_touch_the_device():
     for empty in (dict(rows=0), dict(F=0)):
         assert _norm(**empty) == 0 and _dropout(**empty) == 0
         assert _gradients(**empty) == EINVAL
-    for call in (dict(ldg=-1), dict(ldx=-1), dict(x=0, dx=16), dict(grad=0, dx=16), dict(stats=0, dx=16), dict(drop=_kept(70000), dx=16)):
+    for call in (dict(ldg=-1), dict(ldx=-1), dict(ldx=7, dx=16), dict(ldg=0, dx=16), dict(x=0, dx=16), dict(grad=0, dx=16), dict(stats=0, dx=16), dict(drop=_kept(70000), dx=16)):
         assert _gradients(**call) == EINVAL, call
     assert _gradients(dtype=9, param=9) == EUNSUPPORTED
     assert _gradients() == 0  # nothing wanted
