@@ -87,29 +87,31 @@ __global__ __launch_bounds__(THREADS) void norm_gradients_kernel(NormArgs<T> a) 
     arrived(b);
     for (; r < a.rows; r += step) {
         C h[K][N], g[K][N];
+        Pack<T, N> x[K], d[K];
         const Centre<C> centre(next_mean, next_rstd);
+        row_arrived<T, LANES, K>(next_x, a.x, r * a.ldx, extent_x, lane, F, x);
+        row_arrived<T, LANES, K>(next_g, a.grad, r * a.ldg, extent_g, lane, F, d);
+        ask(r + step < a.rows ? r + step : r);
         C sum = 0, product = 0;
         Draws drawn[K];
         if constexpr (DROP) draw_row<N, LANES>(a.drop.seed, offset, (uint64_t)(r * a.drop.blocks), lane, drawn);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int j = (lane + k * LANES) * N, from = j < F ? j : 0;
-            const auto x = settled<T>(next_x[k], a.x, r * a.ldx + from, extent_x);
-            auto d = settled<T>(next_g[k], a.grad, r * a.ldg + from, extent_g);
             C v[N];
-            normalised<RELU, N>(x.v, centre, w[k], b[k], h[k], v);
-            if constexpr (DROP) d = masked<T, N>(d, drawn[k], a.drop.kept);
+            normalised<RELU>(x[k], centre, w[k], b[k], h[k], v);
+            if constexpr (DROP) d[k] = masked<T, N>(d[k], drawn[k], a.drop.kept);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                g[k][i] = (C)d.v[i];
+                g[k][i] = (C)d[k].v[i];
                 if constexpr (RELU) g[k][i] = v[i] <= 0 ? C(0) : g[k][i];
             }
-            if (j + N > F)  // behind the row's end lies what the next one holds
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            if ((lane + k * LANES) * N + N > F)  // behind the row's end lies what the next one holds
 #pragma unroll
                 for (int i = 0; i < N; ++i)
-                    if (j + i >= F) h[k][i] = g[k][i] = C(0);
-        }
-        ask(r + step < a.rows ? r + step : r);
+                    if ((lane + k * LANES) * N + i >= F) h[k][i] = g[k][i] = C(0);
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -179,7 +181,7 @@ __device__ __forceinline__ void taken(const NormArgs<T> &a, const Pack<T, N> &x,
                                       compute_t<T> (&g)[N]) {
     using C = compute_t<T>;
     C v[N];
-    normalised<RELU, N>(x.v, centre, w, b, h, v);
+    normalised<RELU>(x, centre, w, b, h, v);
     if constexpr (DROP) {
         Draws drawn = draw(a.drop.seed, offset, (uint64_t)(r * a.drop.blocks + j / kDrawn));
         drawn.from<N>((int)(j % kDrawn));
@@ -325,8 +327,8 @@ __global__ __launch_bounds__(kWave) void norm_few_gradients_kernel(NormArgs<T> a
         C w[1], b[1] = {}, hh[1], v[1];
         a.weight.template read<1>(j, a.F, C(1), w);
         if constexpr (RELU) a.bias.template read<1>(j, a.F, C(0), b);
-        const T x[1] = {a.x[r * a.ldx + j]};
-        normalised<RELU, 1>(x, Centre<C>(a.stats[2 * r], a.stats[2 * r + 1]), w, b, hh, v);
+        const Pack<T, 1> x = {{a.x[r * a.ldx + j]}};
+        normalised<RELU>(x, Centre<C>(a.stats[2 * r], a.stats[2 * r + 1]), w, b, hh, v);
         h = hh[0];
         weight = w[0];
         g = (C)a.grad[r * a.ldg + j];

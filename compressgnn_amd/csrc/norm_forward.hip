@@ -11,15 +11,14 @@ namespace {
 template <typename T, int LANES, int K, int THREADS, bool RELU, bool DROP>
 __global__ __launch_bounds__(THREADS) void norm_rows_kernel(NormArgs<T> a) {
     using C = compute_t<T>;
-    constexpr int N = 16 / (int)sizeof(T), GROUPS = THREADS / LANES;
+    constexpr int N = 16 / (int)sizeof(T);
     __shared__ double scratch[LANES > kWave ? THREADS / kWave * 2 : 1];
     const int lane = threadIdx.x % LANES, F = (int)a.F;
-    const int64_t extent = (a.rows - 1) * a.ldx + F;
+    const int64_t step = a.walk.step, extent = (a.rows - 1) * a.ldx + F;
+    const int64_t end = std::min(a.rows, (int64_t)blockIdx.x * a.walk.first + step * a.walk.rounds);
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
     const double inverse_F = 1.0 / (double)F;
-    const int64_t step = a.walk.step;
     int64_t r = (int64_t)blockIdx.x * a.walk.first + threadIdx.x / LANES;
-    const int64_t end = std::min(a.rows, (int64_t)blockIdx.x * a.walk.first + step * a.walk.rounds);
 
     words_t next[K];
     T next_first = T(0);
@@ -46,17 +45,15 @@ __global__ __launch_bounds__(THREADS) void norm_rows_kernel(NormArgs<T> a) {
     for (; r < end; r += step) {
         Pack<T, N> x[K];
         const T first = next_first;
-        const double pivot = (double)first;
+        row_arrived<T, LANES, K>(next, a.x, r * a.ldx, extent, lane, F, x);
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int j = (lane + k * LANES) * N;
-            x[k] = settled<T>(next[k], a.x, r * a.ldx + (j < F ? j : 0), extent);
-            if (j + N > F)  // what lies behind the row's end adds nothing to its sums
+        for (int k = 0; k < K; ++k)
+            if ((lane + k * LANES) * N + N > F)  // what lies behind the row's end adds nothing to its sums
 #pragma unroll
                 for (int i = 0; i < N; ++i)
-                    if (j + i >= F) x[k].v[i] = first;
-        }
+                    if ((lane + k * LANES) * N + i >= F) x[k].v[i] = first;
         ask(r + step < end ? r + step : r);
+        const double pivot = (double)first;
         double sum = 0, squares = 0;
 #pragma unroll
         for (int k = 0; k < K; ++k)
@@ -69,14 +66,13 @@ __global__ __launch_bounds__(THREADS) void norm_rows_kernel(NormArgs<T> a) {
         row_sums<LANES, THREADS>(sum, squares, scratch);
         const Moments m = moments(pivot, sum, squares, inverse_F);
         const Centre<C> centre(m.mean, reciprocal_root(m.variance + a.eps));
-        T *out = a.out + r * a.F;
         Pack<T, N> y[K];
         Draws drawn[K];
         if constexpr (DROP) draw_row<N, LANES>(a.drop.seed, offset, (uint64_t)(r * a.drop.blocks), lane, drawn);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             C h[N], v[N];
-            normalised<RELU, N>(x[k].v, centre, w[k], b[k], h, v);
+            normalised<RELU>(x[k], centre, w[k], b[k], h, v);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 if constexpr (RELU) v[i] = rectified(v[i]);
@@ -92,7 +88,7 @@ __global__ __launch_bounds__(THREADS) void norm_rows_kernel(NormArgs<T> a) {
             a.stats[2 * r + 1] = centre.rstd;
         }
 #pragma unroll
-        for (int k = 0; k < K; ++k) store_columns<T, N>(out, (lane + k * LANES) * N, F, y[k], a.streamed);
+        for (int k = 0; k < K; ++k) store_columns<T, N>(a.out + r * a.F, (lane + k * LANES) * N, F, y[k], a.streamed);
     }
 }
 
@@ -149,7 +145,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs<T> a) 
                 const int64_t j = j0 + k * kStride;
                 const auto x = settled<T>(asked[k], a.x, at + std::min(j, a.F - 1), extent);
                 C h[N], v[N];
-                normalised<RELU, N>(x.v, centre, w[k], b[k], h, v);
+                normalised<RELU>(x, centre, w[k], b[k], h, v);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     if constexpr (RELU) v[i] = rectified(v[i]);
@@ -188,11 +184,11 @@ __global__ __launch_bounds__(kWave) void norm_few_kernel(NormArgs<T> a) {
     }
     const Draws drawn = DROP ? draw(a.drop.seed, drop_offset(a.drop), (uint64_t)r) : Draws{};  // F < 8: one call a row
     for (int64_t j = 0; j < a.F; ++j) {
-        const T one[1] = {x[j]};
+        const Pack<T, 1> one = {{x[j]}};
         C w[1], b[1], h[1], v[1];
         a.weight.template read<1>(j, a.F, C(1), w);
         a.bias.template read<1>(j, a.F, C(0), b);
-        normalised<RELU, 1>(one, centre, w, b, h, v);
+        normalised<RELU>(one, centre, w, b, h, v);
         if constexpr (RELU) v[0] = rectified(v[0]);
         if constexpr (DROP) v[0] = drawn.keeps((int)j, a.drop.kept) ? v[0] * (C)a.drop.scale : C(0);
         a.out[r * a.F + j] = (T)v[0];

@@ -237,6 +237,23 @@ __device__ __forceinline__ void arrived(T &asked) {
     }
 }
 
+// The packs of a row as `ask_within` got them, and, where the row is one of the last and they may run out of the matrix, as
+// asked for.
+template <typename T, int LANES, int K, int N = 16 / (int)sizeof(T)>
+__device__ __forceinline__ void row_arrived(const words_t (&asked)[K], const T *matrix, int64_t at, int64_t extent, int lane, int F, Pack<T, N> (&x)[K]) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) x[k] = __builtin_bit_cast(Pack<T, N>, asked[k]);
+    if (at + LANES * K * N > extent)
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int j = (lane + k * LANES) * N;
+            const int64_t from = at + (j < F ? j : 0);
+            if (from > extent - N)
+#pragma unroll
+                for (int i = 0; i < N; ++i) x[k].v[i] = matrix[from + i < extent ? from + i : extent - 1];
+        }
+}
+
 template <typename T, int N = 16 / (int)sizeof(T)>
 __device__ __forceinline__ Pack<T, N> settled(words_t asked, const T *matrix, int64_t at, int64_t extent) {
     Pack<T, N> p = __builtin_bit_cast(Pack<T, N>, asked);
@@ -536,15 +553,15 @@ struct Centre {
     __device__ __forceinline__ C of(C x) const { return fused(x - near, scale, rest); }
 };
 
-// h = (x - m) r and v = h w + b of N elements.  Forward pass and gradient call this with the same numbers, and with RELU the
+// h = (x - m) r and v = h w + b of a pack.  Forward pass and gradient call this with the same numbers, and with RELU the
 // side of zero that v is on is that of its value in 64 bits: h takes three roundings and v one more, so v is less than
 // 2^-22 (|b| + |v|) off and its sign is certain where |v| > 2^-21 |b|; the few packs that come closer (one of 100,000) are
 // computed again.  A float decision alone would let a sum over a million elements be a whole gradient off now and then.
 template <bool RELU, int N, typename T, typename C>
-__device__ __forceinline__ void normalised(const T (&x)[N], const Centre<C> &centre, const C (&w)[N], const C (&b)[N], C (&h)[N], C (&v)[N]) {
+__device__ __forceinline__ void normalised(const Pack<T, N> &x, const Centre<C> &centre, const C (&w)[N], const C (&b)[N], C (&h)[N], C (&v)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        h[i] = centre.of((C)x[i]);
+        h[i] = centre.of((C)x.v[i]);
         v[i] = fused(h[i], w[i], b[i]);
     }
     if constexpr (RELU && sizeof(C) == 4) {
@@ -559,7 +576,7 @@ __device__ __forceinline__ void normalised(const T (&x)[N], const Centre<C> &cen
             for (int i = 0; i < N; ++i) {
                 float weight = w[i], bias = b[i];
                 asm volatile("" : "+v"(weight), "+v"(bias));  // widened here: not ahead of the rows, in registers of its own
-                const double exact = __builtin_fma(((double)x[i] - centre.mean) * centre.rstd, (double)weight, (double)bias);
+                const double exact = __builtin_fma(((double)x.v[i] - centre.mean) * centre.rstd, (double)weight, (double)bias);
                 if (__builtin_fabsf(v[i]) <= largest * 0x1p-21f) v[i] = (C)exact;
             }
         }
