@@ -258,7 +258,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_dx_kernel(NormArgs<T> 
     }
 }
 
-// Their dw and db: blockIdx.x names the part, `part` rows each, blockIdx.y the columns.  A lane keeps its columns and goes down the rows.
+// Their dw and db: blockIdx.y names the part, `part` rows each, blockIdx.x the columns.  A lane keeps its columns and goes down the rows.
 template <typename T, bool RELU, bool DROP>
 __global__ __launch_bounds__(kBlock) void norm_long_parts_kernel(NormArgs<T> a, int64_t part) {
     using C = compute_t<T>;
@@ -267,9 +267,9 @@ __global__ __launch_bounds__(kBlock) void norm_long_parts_kernel(NormArgs<T> a, 
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
     const int64_t extent_x = (a.rows - 1) * a.ldx + a.F, extent_g = (a.rows - 1) * a.ldg + a.F;
     const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-    const int64_t j = ((int64_t)blockIdx.y * kLanes + lane) * N, from = std::min(j, a.F - 1);
-    const int64_t last = std::min(a.rows, (int64_t)(blockIdx.x + 1) * part);
-    int64_t r = (int64_t)blockIdx.x * part + group;
+    const int64_t j = ((int64_t)blockIdx.x * kLanes + lane) * N, from = std::min(j, a.F - 1);
+    const int64_t last = std::min(a.rows, (int64_t)(blockIdx.y + 1) * part);
+    int64_t r = (int64_t)blockIdx.y * part + group;
     words_t next_x[1] = {}, next_g[1] = {};
     double next_mean = 0, next_rstd = 0;
     auto ask = [&](int64_t row) {
@@ -312,7 +312,7 @@ __global__ __launch_bounds__(kBlock) void norm_long_parts_kernel(NormArgs<T> a, 
                     weight += sums[k][0][i][lane];
                     bias += sums[k][1][i][lane];
                 }
-                C *to = a.partial ? a.partial + (int64_t)blockIdx.x * 2 * a.F : nullptr;
+                C *to = a.partial ? a.partial + (int64_t)blockIdx.y * 2 * a.F : nullptr;
                 leave_sum<T>(to, a.dweight, a.weight.wide, j + i, weight * dropped);
                 leave_sum<T>(to ? to + a.F : nullptr, a.dbias, a.weight.wide, j + i, bias * dropped);
             }
@@ -410,7 +410,7 @@ int gradients_launch(const NormArgs<T> &a, const RowShape &shape, int64_t parts,
         if (int rc = check_launch("layer_norm_backward")) return rc;
     }
     if (a.partial || a.dweight || a.dbias) {
-        const dim3 grid((unsigned)parts, (unsigned)ceil_div(a.F, (int64_t)kLanes * 16 / (int64_t)sizeof(T)));
+        const dim3 grid((unsigned)ceil_div(a.F, (int64_t)kLanes * 16 / (int64_t)sizeof(T)), (unsigned)parts);
         hipLaunchKernelGGL((norm_long_parts_kernel<T, RELU, DROP>), grid, dim3(kBlock), 0, stream, a, ceil_div(a.rows, parts));
     }
     return check_launch("layer_norm_backward");

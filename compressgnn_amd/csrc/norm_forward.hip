@@ -1,6 +1,8 @@
 // Layer norm of node rows, with the ReLU and the dropout behind it in the same pass:
 //
 //   m = sum x / F, v = sum (x - m)^2 / F, r = 1 / sqrt(v + eps), out = drop(relu((x - m) r w + b))
+#include <limits>
+
 #include "rows.h"
 
 namespace cgnn {
@@ -236,7 +238,8 @@ extern "C" int cgnn_layer_norm(int64_t rows, int64_t F, int dtype, int param_dty
                                const void *weight, const void *bias, double eps, int relu, const cgnn_drop *drop, void *out,
                                double *stats, cgnn_stream_t stream) {
     CGNN_REQUIRE(rows >= 0 && F >= 0 && (rows <= 1 || ldx >= F), "cgnn_layer_norm: bad size");
-    CGNN_REQUIRE(eps >= 0, "cgnn_layer_norm: eps must not be negative");
+    CGNN_REQUIRE(F < ((int64_t)1 << 31) - 65536, "cgnn_layer_norm: a row must be shorter than 2^31 elements");
+    CGNN_REQUIRE(eps >= 0 && eps <= std::numeric_limits<double>::max(), "cgnn_layer_norm: eps must be finite and not negative");
     CGNN_REQUIRE(param_dtype == dtype || (param_dtype == CGNN_F32 && dtype != CGNN_F64),
                  "cgnn_layer_norm: parameters have the type of the rows, or f32 for 16-bit rows");
     if (drop) CGNN_REQUIRE_DROP("cgnn_layer_norm", drop);

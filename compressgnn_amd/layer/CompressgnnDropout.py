@@ -57,7 +57,7 @@ class Masks:
         if x.is_cuda and torch.cuda.is_current_stream_capturing():
             if self.replays.device != x.device:
                 raise RuntimeError("the module is on %s and x on %s: move it there before the capture" % (self.replays.device, x.device))
-            counter = self.replays.clone()
+            counter = self.replays + 0
             self.replays += 1
             return self.seed, self.CAPTURED, counter
         self.calls += 1

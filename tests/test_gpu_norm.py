@@ -300,6 +300,44 @@ def test_rows_beyond_32_bit_offsets():
     assert torch.equal(dx[at], torch.autograd.grad(small_out, small, x[at])[0])
 
 
+@pytest.mark.parametrize("rows,dtype", [((1 << 21) + 77, BF16), (300007, F32)])
+def test_matrices_beyond_the_caches(rows, dtype):
+    """Whole lines, more of them than the last-level cache holds: other stores, and from a gigabyte on another way through the rows."""
+    width = 256
+    gen = torch.Generator(DEV).manual_seed(1)
+    x, grad = (torch.randn(rows, width, device=DEV, generator=gen, dtype=F32).to(dtype) for _ in range(2))
+    w, b = parameters(width, F32, 1)
+    out = dropout(x, 0.5, 3, 1)
+    zero = torch.zeros((), dtype=dtype, device=DEV)
+    assert bool(((out == zero) | (out == x * 2)).all())
+    at = torch.cat([torch.arange(0, 300), torch.arange(rows // 2, rows // 2 + 100), torch.arange(rows - 300, rows)]).to(DEV)
+    for first, last in ((0, 300), (rows // 2, rows // 2 + 100), (rows - 300, rows)):
+        kept = torch.from_numpy(mask(last - first, width, 0.5, 3, 1, first_row=first)).to(DEV)
+        assert torch.equal(out[first:last], torch.where(kept, x[first:last] * 2, zero))
+    del out
+    l = leaves(x, w, b)
+    out = norm_act_dropout(*l, 1e-5, "relu")
+    dx, dw, db = torch.autograd.grad(out, l, grad)
+    small = leaves(x[at], w, b)
+    small_out = norm_act_dropout(*small, 1e-5, "relu")
+    assert torch.equal(out[at], small_out)
+    assert torch.equal(dx[at], torch.autograd.grad(small_out, small[0], grad[at])[0])
+    off, sums = 0.0, [torch.zeros(width, dtype=F64, device=DEV) for _ in range(4)]
+    for first in range(0, rows, 1 << 18):  # every row against 64 bits, the sums against theirs
+        X, G = x[first:first + (1 << 18)].double(), grad[first:first + (1 << 18)].double()
+        h = X - X.mean(1, keepdim=True)
+        h = h / torch.sqrt((h * h).mean(1, keepdim=True) + 1e-5)
+        v = h * w.double() + b.double()
+        G = G * (v > 0)
+        off = max(off, float((out[first:first + (1 << 18)].double() - v.clamp_min(0)).abs().max()))
+        for total, part in zip(sums, (G * h, (G * h).abs(), G, G.abs())):
+            total += part.sum(0)
+    # a value of at most 32: half a step of its type and a few of float
+    assert off <= 32 * ({BF16: 2.0 ** -8, F32: 2.0 ** -24}[dtype] + 8 * 2.0 ** -24)
+    for got, want, size in ((dw, sums[0], sums[1]), (db, sums[2], sums[3])):
+        assert bool(((got.double() - want).abs() <= (1024 + 68) * 2.0 ** -24 * size).all())
+
+
 # -------------------------------------------------------------- streams, graphs, autograd --
 def test_other_streams_and_repeated_calls_give_the_same_bits():
     x, grad = features(3000, 130, F32, 1), features(3000, 130, F32, 2)

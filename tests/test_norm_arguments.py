@@ -116,8 +116,8 @@ def test_entry_points_check_before_they_touch_the_device():
     """Every call here is refused, or has nothing to do, on the host: no address in it is ever read."""
     for call in (dict(rows=-1), dict(F=-1), dict(ldx=-1), dict(ldx=7), dict(x=0), dict(out=0), dict(drop=_kept(-1)), dict(drop=_kept(65537))):
         assert _norm(**call) == EINVAL and _dropout(**call) == EINVAL, call
-    assert _dropout(drop=None) == EINVAL
-    for eps in (-1e-9, float("nan")):
+    assert _dropout(drop=None) == EINVAL and _norm(F=1 << 31, ldx=1 << 31) == EINVAL and _gradients(F=1 << 31, ldx=1 << 31, ldg=1 << 31, dx=16) == EINVAL
+    for eps in (-1e-9, float("nan"), float("inf")):
         assert _norm(eps=eps) == EINVAL
     assert _norm(dtype=4, param=4) == EUNSUPPORTED and _dropout(dtype=-1) == EUNSUPPORTED
     for dtype, param in ((0, 1), (1, 0), (2, 3), (3, 1)):
