@@ -46,7 +46,8 @@ __global__ __launch_bounds__(THREADS) void norm_gradients_kernel(NormArgs<T> a) 
     using C = compute_t<T>;
     constexpr int N = 16 / (int)sizeof(T), GROUPS = THREADS / LANES, WAVES = THREADS / kWave;
     constexpr int COLUMNS = LANES * K * N;  // that the lanes have room for
-    __shared__ C scratch[LANES > kWave ? WAVES * 2 : WAVES * COLUMNS];
+    __shared__ C scratch[LANES > kWave ? WAVES * 4 : WAVES * COLUMNS];
+    bool odd = false;
     const int lane = threadIdx.x % LANES, F = (int)a.F;
     const int64_t extent_x = (a.rows - 1) * a.ldx + F, extent_g = (a.rows - 1) * a.ldg + F;
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
@@ -123,7 +124,7 @@ __global__ __launch_bounds__(THREADS) void norm_gradients_kernel(NormArgs<T> a) 
                 product = fused(g[k][i], h[k][i], product);
             }
         if (a.dx) {
-            row_sums<LANES, THREADS>(sum, product, scratch);
+            row_sums<LANES, THREADS>(sum, product, scratch, odd);
             const C c1 = sum * inverse_F, c2 = product * inverse_F, scale = centre.scale * dropped;
             Pack<T, N> dx[K];
 #pragma unroll
@@ -201,7 +202,8 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_dx_kernel(NormArgs<T> 
     using C = compute_t<T>;
     constexpr int N = 16 / (int)sizeof(T), PACKS = sizeof(T) == 2 ? 1 : 2;  // as many as the registers hold
     constexpr int64_t kStride = (int64_t)kLongThreads * N;
-    __shared__ C scratch[kLongThreads / kWave * 2];
+    __shared__ C scratch[kLongThreads / kWave * 4];
+    bool odd = false;
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
     const int64_t extent_x = (a.rows - 1) * a.ldx + a.F, extent_g = (a.rows - 1) * a.ldg + a.F;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
@@ -242,7 +244,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_dx_kernel(NormArgs<T> 
                 }
             }
         }
-        row_sums<kLongThreads, kLongThreads>(sum, product, scratch);
+        row_sums<kLongThreads, kLongThreads>(sum, product, scratch, odd);
         const C c1 = sum / (C)a.F, c2 = product / (C)a.F, scale = centre.scale * (DROP ? (C)a.drop.scale : C(1));
         for (int64_t j0 = (int64_t)threadIdx.x * N; j0 < a.F; j0 += PACKS * kStride) {
             ask(j0);

@@ -14,7 +14,8 @@ template <typename T, int LANES, int K, int THREADS, bool RELU, bool DROP>
 __global__ __launch_bounds__(THREADS) void norm_rows_kernel(NormArgs<T> a) {
     using C = compute_t<T>;
     constexpr int N = 16 / (int)sizeof(T);
-    __shared__ double scratch[LANES > kWave ? THREADS / kWave * 2 : 1];
+    __shared__ double scratch[LANES > kWave ? THREADS / kWave * 4 : 1];
+    bool odd = false;
     const int lane = threadIdx.x % LANES, F = (int)a.F;
     const int64_t step = a.walk.step, extent = (a.rows - 1) * a.ldx + F;
     const int64_t end = std::min(a.rows, (int64_t)blockIdx.x * a.walk.first + step * a.walk.rounds);
@@ -65,7 +66,7 @@ __global__ __launch_bounds__(THREADS) void norm_rows_kernel(NormArgs<T> a) {
                 sum += d;
                 squares = __builtin_fma(d, d, squares);
             }
-        row_sums<LANES, THREADS>(sum, squares, scratch);
+        row_sums<LANES, THREADS>(sum, squares, scratch, odd);
         const Moments m = moments(pivot, sum, squares, inverse_F);
         const Centre<C> centre(m.mean, reciprocal_root(m.variance + a.eps));
         Pack<T, N> y[K];
@@ -100,7 +101,8 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs<T> a) 
     using C = compute_t<T>;
     constexpr int N = 16 / (int)sizeof(T);
     constexpr int64_t kStride = (int64_t)kLongThreads * N;
-    __shared__ double scratch[kLongThreads / kWave * 2];
+    __shared__ double scratch[kLongThreads / kWave * 4];
+    bool odd = false;
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
     const int64_t extent = (a.rows - 1) * a.ldx + a.F;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
@@ -127,7 +129,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs<T> a) 
                 }
             }
         }
-        row_sums<kLongThreads, kLongThreads>(sum, squares, scratch);
+        row_sums<kLongThreads, kLongThreads>(sum, squares, scratch, odd);
         const Moments m = moments(pivot, sum, squares, 1.0 / (double)a.F);
         const Centre<C> centre(m.mean, reciprocal_root(m.variance + a.eps));
         if (a.stats && threadIdx.x == 0) {

@@ -443,26 +443,28 @@ __device__ __forceinline__ A sum_over_groups(A v) {
 }
 
 // Two sums over the lanes of a row: those of a group, or of the whole workgroup (LANES == THREADS > a wave), whose waves
-// leave theirs in `scratch` (two elements a wave) and add them in their order.
+// leave theirs in `scratch` and add them in their order.  `scratch`: two halves of two elements a wave, of which a row takes the one that the
+// row before did not: whoever writes a half has passed the barrier of the row between, and so has everyone who read it.
 template <int LANES, int THREADS, typename A>
-__device__ __forceinline__ void row_sums(A &first, A &second, A *scratch) {
+__device__ __forceinline__ void row_sums(A &first, A &second, A *scratch, bool &odd) {
     constexpr int kGroup = LANES < kWave ? LANES : kWave;
     first = group_sum<kGroup>(first);
     second = group_sum<kGroup>(second);
     if constexpr (LANES > kWave) {
         static_assert(LANES == THREADS, "a row is a lane group's or the whole workgroup's");
-        __syncthreads();  // the last sums' readers are done
+        A *half = scratch + (odd ? THREADS / kWave * 2 : 0);
+        odd = !odd;
         if (threadIdx.x % kWave == 0) {
-            scratch[threadIdx.x / kWave * 2] = first;
-            scratch[threadIdx.x / kWave * 2 + 1] = second;
+            half[threadIdx.x / kWave * 2] = first;
+            half[threadIdx.x / kWave * 2 + 1] = second;
         }
         __syncthreads();
-        first = scratch[0];
-        second = scratch[1];
+        first = half[0];
+        second = half[1];
 #pragma unroll
         for (int w = 1; w < THREADS / kWave; ++w) {
-            first += scratch[2 * w];
-            second += scratch[2 * w + 1];
+            first += half[2 * w];
+            second += half[2 * w + 1];
         }
     }
 }
@@ -587,8 +589,9 @@ __device__ __forceinline__ void normalised(const Pack<T, N> &x, const Centre<C> 
 // How a row is spread: packs of 16 bytes over `lanes` lanes, `packs` on each; a workgroup has `threads`.  0 lanes: too long for
 // registers.  The fewest places for the row's packs among powers of two with two or three packs a lane: several packs share the
 // additions across the lanes and what is computed once a row, and leave loads enough in flight for a few waves a SIMD.
-// Rows of 129 to 256 packs are one wave's, four packs a lane, in the forward pass (2,048 bfloat16 features, 43,945 rows: 75
-// against 80 us with a pack a lane of four waves); in the gradient, whose sums take registers too, four waves' with a pack a lane (124
+// Rows of 193 to 320 packs are one wave's, four or five packs a lane, in the forward pass (2,048 bfloat16 features, 43,945 rows: 75
+// against 80 us with a pack a lane of four waves; 1,200 float32 features, 40,000 rows: 76 against 87 with two; beyond, 2,048 of
+// float32, 4,096 rows, 19 against 14); in the gradient, whose sums take registers too, four waves' with a pack a lane (124
 // against 144).  Of a 16-bit row a pack has eight columns, and the lanes of
 // 512 have registers for two packs in the gradient, not four.
 struct RowShape {
@@ -604,7 +607,8 @@ inline RowShape row_shape(int64_t F, size_t element, bool gradient) {
         if (lanes > kWave || packs <= 3 * (lanes / 2)) return {lanes / 2, 3, kBlock};
         return {lanes, 2, kBlock};
     }
-    if (packs <= 256) return gradient ? RowShape{256, 1, 256} : RowShape{64, 4, 256};
+    if (packs <= 320 && !gradient) return {64, packs <= 256 ? 4 : 5, 256};
+    if (packs <= 256) return {256, 1, 256};
     if (packs <= 768) return {256, packs <= 512 ? 2 : 3, 256};
     return {512, packs <= 1024 ? 2 : packs <= 1536 ? 3 : 4, 512};
 }
@@ -645,7 +649,7 @@ int with_row_shape(const RowShape &s, F &&run) {
         case 32: return s.packs == 2 ? run(ShapeTag<32, 2, 256>()) : run(ShapeTag<32, 3, 256>());
         case 64:
             if constexpr (!GRADIENT)
-                if (s.packs == 4) return run(ShapeTag<64, 4, 256>());
+                if (s.packs > 3) return s.packs == 4 ? run(ShapeTag<64, 4, 256>()) : run(ShapeTag<64, 5, 256>());
             return s.packs == 2 ? run(ShapeTag<64, 2, 256>()) : run(ShapeTag<64, 3, 256>());
         case 256:
             if constexpr (GRADIENT)
