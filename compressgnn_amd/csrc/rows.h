@@ -591,7 +591,7 @@ __device__ __forceinline__ void normalised(const Pack<T, N> &x, const Centre<C> 
 // additions across the lanes and what is computed once a row, and leave loads enough in flight for a few waves a SIMD.
 // Rows of 193 to 320 packs are one wave's, four or five packs a lane, in the forward pass (2,048 bfloat16 features, 43,945 rows: 75
 // against 80 us with a pack a lane of four waves; 1,200 float32 features, 40,000 rows: 76 against 87 with two; beyond, 2,048 of
-// float32, 4,096 rows, 19 against 14); in the gradient, whose sums take registers too, four waves' with a pack a lane (124
+// float32, 4,096 rows, 19 against 14), then up to 384 packs two waves' (2,800 bfloat16 features, 40,000 rows, 90 against 99 us); in the gradient, whose sums take registers too, four waves' with a pack a lane (124
 // against 144).  Of a 16-bit row a pack has eight columns, and the lanes of
 // 512 have registers for two packs in the gradient, not four.
 struct RowShape {
@@ -608,6 +608,7 @@ inline RowShape row_shape(int64_t F, size_t element, bool gradient) {
         return {lanes, 2, kBlock};
     }
     if (packs <= 320 && !gradient) return {64, packs <= 256 ? 4 : 5, 256};
+    if (packs <= 384 && !gradient) return {128, 3, 128};
     if (packs <= 256) return {256, 1, 256};
     if (packs <= 768) return {256, packs <= 512 ? 2 : 3, 256};
     return {512, packs <= 1024 ? 2 : packs <= 1536 ? 3 : 4, 512};
@@ -651,6 +652,8 @@ int with_row_shape(const RowShape &s, F &&run) {
             if constexpr (!GRADIENT)
                 if (s.packs > 3) return s.packs == 4 ? run(ShapeTag<64, 4, 256>()) : run(ShapeTag<64, 5, 256>());
             return s.packs == 2 ? run(ShapeTag<64, 2, 256>()) : run(ShapeTag<64, 3, 256>());
+        case 128:
+            if constexpr (!GRADIENT) return run(ShapeTag<128, 3, 128>());
         case 256:
             if constexpr (GRADIENT)
                 if (s.packs == 1) return run(ShapeTag<256, 1, 256>());

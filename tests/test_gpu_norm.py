@@ -16,7 +16,7 @@ TYPES = [F32, F64, F16, BF16]
 # one row and one column, ends inside and at the packs and lane groups of every type, rows of many waves, rows longer than any group holds
 SHAPES = [(1, 1), (3, 1), (5, 2), (2, 3), (300, 4), (7, 5), (1000, 7), (65, 8), (13, 9), (40, 15), (257, 16), (33, 17), (100, 31), (64, 33),
           (1000, 47), (129, 64), (31, 65), (2708, 128), (50, 129), (100, 255), (300, 256), (41, 257), (9, 511), (20, 513), (33, 602),
-          (5, 1023), (6, 1025), (700, 1024), (3, 1030), (17, 2047), (4, 2050), (3, 4096), (2, 4103), (5, 8191), (2, 8200), (1, 12345),
+          (5, 1023), (6, 1025), (700, 1024), (3, 1030), (5, 1500), (7, 1200), (17, 2047), (4, 2050), (4, 2600), (5, 3050), (3, 4096), (2, 4103), (5, 8191), (2, 8200), (1, 12345),
           (2, 16384), (3, 20001)]
 
 
@@ -241,6 +241,17 @@ def test_rows_that_hold_one_value(width):
     x[1:] = features(3, width, F32, 1)
     out = layer_norm(x, w, b, 0.0)
     assert torch.isnan(out[0]).all() and (width == 1 or torch.isfinite(out[1:]).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_of_one_element_have_no_gradient(dtype):
+    """Nothing of a row is left when its mean is taken away: zeros, not the rest of a cancellation."""
+    for rows in (1, 3, 500, 70001):
+        x, grad = features(rows, 1, dtype, 3), features(rows, 1, dtype, 4)
+        l = leaves(x, *parameters(1, dtype, 2))
+        for activation, p in ((None, 0.0), ("relu", 0.4)):
+            dx, dw, _ = torch.autograd.grad(norm_act_dropout(*l, 1e-5, activation, p, 5), l, grad)
+            assert not dx.any() and not dw.any()
 
 
 @pytest.mark.parametrize("dtype", TYPES)
