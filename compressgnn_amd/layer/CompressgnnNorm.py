@@ -15,6 +15,7 @@ import compressgnn_runtime as _native
 from CompressgnnDropout import Masks
 
 _ACTIVATIONS = (None, 'relu')
+_layer_norm = _native.layer_norm
 
 
 class _Normed(torch.autograd.Function):
@@ -43,13 +44,14 @@ def norm_act_dropout(x, weight=None, bias=None, eps=1e-5, activation=None, p=0.0
     if activation not in _ACTIVATIONS:
         raise ValueError("activation must be None or 'relu'")
     relu = activation is not None
-    out = _native.layer_norm(x, weight, bias, eps, relu, p, seed, offset, counter)
+    out = _layer_norm(x, weight, bias, eps, relu, p, seed, offset, counter)
     return _Normed.apply(x, weight, bias, eps, relu, p, seed, offset, counter) if out is None else out
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(variance + eps) * weight + bias over the last dimension of x."""
-    return norm_act_dropout(x, weight, bias, eps)
+    out = _layer_norm(x, weight, bias, eps)
+    return norm_act_dropout(x, weight, bias, eps) if out is None else out
 
 
 class Compressgnn_LayerNorm(Masks, torch.nn.Module):

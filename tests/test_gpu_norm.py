@@ -17,7 +17,9 @@ TYPES = [F32, F64, F16, BF16]
 SHAPES = [(1, 1), (3, 1), (5, 2), (2, 3), (300, 4), (7, 5), (1000, 7), (65, 8), (13, 9), (40, 15), (257, 16), (33, 17), (100, 31), (64, 33),
           (1000, 47), (129, 64), (31, 65), (2708, 128), (50, 129), (100, 255), (300, 256), (41, 257), (9, 511), (20, 513), (33, 602),
           (5, 1023), (6, 1025), (700, 1024), (3, 1030), (5, 1500), (7, 1200), (17, 2047), (4, 2050), (4, 2600), (5, 3050), (3, 4096), (2, 4103), (5, 8191), (2, 8200), (1, 12345),
-          (2, 16384), (3, 20001)]
+          (2, 16384), (3, 20001),
+          # more rows than lanes at once, each width of the above but the longest
+          (270000, 5), (70003, 17), (40000, 40), (20000, 70), (20000, 130), (9000, 200), (5000, 390), (2600, 601), (1100, 1100)]
 
 
 def features(rows, width, dtype, seed, offset=0.3):
