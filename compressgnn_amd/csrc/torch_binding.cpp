@@ -11,6 +11,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <hip/hip_runtime_api.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -2370,6 +2371,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("reconstruct", &reconstruct, "act(reps[index] + bias) with its gradients", py::arg("reps"), py::arg("index"),
           py::arg("bias"), py::arg("relu"), py::arg("members") = py::none());
     m.def("column_sums", &column_sums, "sum over the rows of a matrix");
+    m.def("in_backward", [] { return torch::autograd::get_current_graph_task_id() != -1; },
+          "whether this thread is inside a backward pass");
     m.def("dropout", &dropout, "elements dropped by position, with the gradient", py::arg("x"), py::arg("p"), py::arg("seed"),
           py::arg("offset") = 0, py::arg("counter") = py::none());
     m.def("layer_norm", &layer_norm, "layer norm, ReLU and dropout of rows in one pass, with the gradients", py::arg("x"),

@@ -42,7 +42,9 @@ class Masks:
     """The masks of a module, one after the other: each is named by the module's seed and the number of the call.
 
     Calls under a stream capture are numbered on the device, by a counter that the captured work itself
-    counts up, and lie in a range of their own; the module has to be on the device of the rows before."""
+    counts up, and lie in a range of their own; the module has to be on the device of the rows before.  A copy of a module
+    draws the masks that the module draws.  A forward pass computed again in a backward one (activation checkpointing) would draw
+    other masks than the first time and is refused: there the functions, whose masks have names, serve."""
 
     CAPTURED = 1 << 62  # offsets of captured calls begin here
 
@@ -50,10 +52,13 @@ class Masks:
         # of torch's own generator where none is given: torch.manual_seed fixes it, and no two modules share masks
         self.seed = int(torch.randint(1 << 62, (1,))) if seed is None else int(seed)
         self.calls = 0
-        self.register_buffer('replays', torch.zeros(1, dtype=torch.int64), persistent=False)
+        self.register_buffer('replays', torch.zeros(1, dtype=torch.int64))
 
     def _next_mask(self, x):
         """(seed, offset, counter) of a call on x"""
+        if _native.in_backward():
+            raise RuntimeError("a call within a backward pass would draw another mask than the forward pass did; call dropout or "
+                               "norm_act_dropout with a seed and an offset where activations are computed again")
         if x.is_cuda and torch.cuda.is_current_stream_capturing():
             if self.replays.device != x.device:
                 raise RuntimeError("the module is on %s and x on %s: move it there before the capture" % (self.replays.device, x.device))
@@ -71,8 +76,8 @@ class Masks:
 
 
 class Compressgnn_Dropout(Masks, torch.nn.Module):
-    """dropout(x, p) in training, x itself otherwise.  seed: fixes the masks; its own and the number of calls so far
-    travel with the state dict, so that training resumed from one draws the masks it would have drawn."""
+    """dropout(x, p) in training, x itself otherwise.  seed: fixes the masks; its own and the numbers of calls so far, captured
+    ones too, travel with the state dict, so that training resumed from one draws the masks it would have drawn."""
 
     def __init__(self, p=0.5, seed=None):
         super().__init__()

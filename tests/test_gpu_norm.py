@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import compressgnn_runtime as rt
 from compressgnn_amd import abi
@@ -550,6 +551,38 @@ def test_modules():
     assert torch.equal(norm(x), norm_act_dropout(x, norm.weight, norm.bias, 1e-5, "relu"))
     plain = Compressgnn_LayerNorm(24, affine=False, dtype=F64)
     assert torch.equal(plain(x.double()), layer_norm(x.double()))
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_activations_computed_again(reentrant):
+    """Masks with names are the same the second time; a module, which counts its calls, refuses the second one."""
+    x, grad = features(90, 40, F32, 1), features(90, 40, F32, 2)
+    w, b = parameters(40, F32, 1)
+
+    def block(x, w, b):
+        return dropout(norm_act_dropout(x, w, b, 1e-5, "relu", 0.25, 3, 1), 0.5, 3, 2)
+
+    l, k = leaves(x, w, b), leaves(x, w, b)
+    want = torch.autograd.grad(block(*l), l, grad)
+    out = torch.utils.checkpoint.checkpoint(block, *k, use_reentrant=reentrant)
+    out.backward(grad)
+    assert all(torch.equal(t.grad, g) for t, g in zip(k, want))
+    drop, norm = Compressgnn_Dropout(0.5, seed=4).to(DEV), Compressgnn_LayerNorm(40, p=0.5).to(DEV)
+    for module in (drop, norm, lambda x: drop(x).square()):
+        (k,) = leaves(x)
+        calls = drop.calls
+        out = torch.utils.checkpoint.checkpoint(module, k, use_reentrant=reentrant)
+        if module is drop and not reentrant:  # keeps no tensor, so nothing is computed again
+            out.backward(grad)
+            assert torch.equal(k.grad, dropout(grad, 0.5, 4, calls))
+            continue
+        with pytest.raises(RuntimeError, match="within a backward pass"):
+            out.backward(grad)
+    plain = Compressgnn_LayerNorm(40, activation="relu").to(DEV)
+    (l,), (k,) = leaves(x), leaves(x)
+    plain(l).backward(grad)
+    torch.utils.checkpoint.checkpoint(plain, k, use_reentrant=reentrant).backward(grad)
+    assert torch.equal(l.grad, k.grad)
 
 
 def test_the_fused_operator_is_the_two_in_a_row():

@@ -81,6 +81,33 @@ def test_state_dict_holds_the_place_in_the_masks():
     assert Compressgnn_Dropout(0.5, seed=(1 << 63) - 1).state_dict()["_extra_state"][0] == (1 << 63) - 1
 
 
+def test_the_place_among_captured_calls_travels_too():
+    a, b = Compressgnn_LayerNorm(4, p=0.5), Compressgnn_LayerNorm(4, p=0.5)
+    a.replays.fill_(11)
+    b.load_state_dict(a.state_dict())
+    assert b.replays.tolist() == [11]
+
+
+def test_a_module_draws_no_mask_in_a_backward_pass():
+    """What is computed again there would be another function than the one whose gradient is asked for."""
+    drop = Compressgnn_Dropout(0.5, seed=1)
+
+    class Again(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return x.clone()
+
+        @staticmethod
+        def backward(ctx, grad):
+            drop._next_mask(grad)
+            return grad
+
+    drop._next_mask(torch.zeros(1))
+    with pytest.raises(RuntimeError, match="within a backward pass"):
+        Again.apply(torch.zeros(1, requires_grad=True)).backward()
+    assert drop.calls == 1
+
+
 def _norm(**changed):
     call = dict(rows=4, F=8, dtype=0, param=0, ldx=8, eps=1e-5, drop=None, x=16, out=16)
     call.update(changed)
