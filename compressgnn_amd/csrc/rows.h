@@ -601,20 +601,21 @@ struct RowShape {
 
 // The same where the chip has lanes enough for about all packs at once, forward: there the time is that of one row's chain of loads
 // and additions, and a pack a lane makes it shortest (257 bfloat16 features: one row 3.0 against 5.5 us, 8,192 rows 8.3 against 9.6;
-// 1,000: one row 3.0 against 4.2, 4,096 rows 9.9 against 12.6; 2,400: 512 rows 6.9 against 9.0, 1,024 rows 9.8 against 9.4, and
-// 8,192 rows, beyond the limit, 27 against 25).
+// 1,000: one row 3.0 against 4.2, 4,096 rows 9.9 against 12.6).  16-bit rows of more than 256 packs, whose columns cost most, take it for
+// four times as many rows (float32 parameters: 2,400 float16 features, 1,500 rows 12 against 22 us, 3,000 18 against 23; 4,096 features,
+// 2,048 rows 17 against 21, 4,096 rows 23 against 25, with float16 ones 23 against 22; beyond the limit 8,192 rows 35 against 33).
 constexpr int64_t kAtOnce = 1 << 19;
 
 inline RowShape spread_shape(int64_t packs) {
     if (packs > 512) return {0, 0, 0};
-    if (packs > 128) return {256, packs <= 256 ? 1 : 2, 256};
-    return {pow2_ceil(packs), 1, packs <= kWave ? kBlock : 128};
+    return {pow2_ceil(packs), 1, std::max(pow2_ceil(packs), packs > kWave ? 128 : kBlock)};
 }
 
 inline RowShape row_shape(int64_t rows, int64_t F, size_t element, bool gradient) {
     const int64_t packs = ceil_div(F, 16 / (int64_t)element);
     const RowShape spread = spread_shape(packs);
-    if (!gradient && spread.lanes && rows * spread.lanes * spread.packs <= kAtOnce) return spread;
+    const int64_t at_once = element == 2 && packs > 256 ? 4 * kAtOnce : kAtOnce;
+    if (!gradient && spread.lanes && rows * spread.lanes <= at_once) return spread;
     if (packs > (gradient && element == 2 ? 1024 : 2048)) return {0, 0, 0};
     if (packs <= 3) return {1, (int)packs, kBlock};
     if (packs <= 192) {
@@ -690,6 +691,8 @@ int with_row_shape(const RowShape &s, F &&run) {
             if (s.packs == 1) return run(ShapeTag<256, 1, 256>());
             return s.packs == 2 ? run(ShapeTag<256, 2, 256>()) : run(ShapeTag<256, 3, 256>());
         default:
+            if constexpr (!GRADIENT)
+                if (s.packs == 1) return run(ShapeTag<512, 1, 512>());
             if constexpr (!GRADIENT || sizeof(T) > 2)
                 if (s.packs > 2) return s.packs == 3 ? run(ShapeTag<512, 3, 512>()) : run(ShapeTag<512, 4, 512>());
             return run(ShapeTag<512, 2, 512>());

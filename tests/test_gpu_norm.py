@@ -20,7 +20,8 @@ SHAPES = [(1, 1), (3, 1), (5, 2), (2, 3), (300, 4), (7, 5), (1000, 7), (65, 8), 
           (5, 1023), (6, 1025), (700, 1024), (3, 1030), (5, 1500), (7, 1200), (17, 2047), (4, 2050), (4, 2600), (5, 3050), (3, 4096), (2, 4103), (5, 8191), (2, 8200), (1, 12345),
           (2, 16384), (3, 20001),
           # more rows than lanes at once, each width of the above but the longest
-          (270000, 5), (70003, 17), (40000, 40), (20000, 70), (20000, 130), (9000, 200), (5000, 390), (2600, 601), (1100, 1100)]
+          (270000, 5), (70003, 17), (40000, 40), (20000, 70), (20000, 130), (9000, 200), (5000, 390), (2600, 601), (1100, 1100), (1030, 700),
+          (1030, 900)]
 
 
 def features(rows, width, dtype, seed, offset=0.3):
@@ -526,6 +527,25 @@ def test_no_rows_and_no_columns():
             assert out.shape == x.shape
             dx, dw, db = torch.autograd.grad(out, (x, w, b), torch.zeros_like(out))
             assert dx.shape == x.shape and dw.shape == w.shape and not dw.any() and not db.any()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("width", [2100, 2700, 3500])
+def test_many_wide_16_bit_rows_are_what_few_are(width, dtype):
+    """Few rows, whose values the formulas check above, are spread over more lanes.  Two roundings of half a step each, of values that are
+    2^-20 of the bias apart at most; below the least normal number of float16 half a step is 2^-25."""
+    rows, few = 4100, 200
+    x = features(rows, width, dtype, 1)
+    w, b = parameters(width, F32, 1)
+
+    def near(many, one):
+        bound = torch.finfo(dtype).eps * one.double().abs() + 2.0 ** -20 * b.abs().max().double() + 2.0 ** -24
+        assert ((many.double() - one.double()).abs() <= bound).all()
+
+    call = (w, b, 1e-5, "relu")
+    near(norm_act_dropout(x, *call, 0.5, 3, 1)[:few], norm_act_dropout(x[:few], *call, 0.5, 3, 1))
+    near(norm_act_dropout(x, *call)[-few:], norm_act_dropout(x[-few:], *call))
+    near(layer_norm(x, w, b)[-few:], layer_norm(x[-few:], w, b))
 
 
 # ---------------------------------------------------------------------------- modules --
