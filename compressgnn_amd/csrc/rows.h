@@ -288,12 +288,12 @@ __device__ __forceinline__ void store_pack(T *row, int64_t j, int64_t F, const P
 }
 
 // 16 bytes, past the caches where they are not read again before they would be gone from there.  In assembly: of two stores that differ
-// in nothing else the compiler makes one, the plain one; and what it knows of stores of more than 8 bytes has to be said too, that their
-// registers may be written again one step later at the earliest.
+// in nothing else the compiler makes one, the plain one; and what it knows of stores of more than 8 bytes has to be said too: gfx950
+// reads their data late, and the vector ALU may write those registers again two wait states behind the store at the earliest.
 template <typename T, int N>
 __device__ __forceinline__ void store_whole(T *to, const Pack<T, N> &p, bool streamed) {
     if (streamed)
-        asm volatile("global_store_dwordx4 %0, %1, off nt\n\ts_nop 0" : : "v"(to), "v"(__builtin_bit_cast(words_t, p)) : "memory");
+        asm volatile("global_store_dwordx4 %0, %1, off nt\n\ts_nop 1" : : "v"(to), "v"(__builtin_bit_cast(words_t, p)) : "memory");
     else
         *reinterpret_cast<Pack<T, N> *>(to) = p;
 }
