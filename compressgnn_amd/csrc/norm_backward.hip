@@ -368,33 +368,36 @@ __global__ __launch_bounds__(kWave) void norm_few_gradients_kernel(NormArgs<T> a
 
 // The parts' sums, added up in 64 bits in an order that the number of parts fixes: column c < F of the weight's gradient, then
 // the bias's.  Sixteen columns a workgroup: as many lines of 64 bytes in flight as it has lane groups (256 to 768 parts of up to
-// 602 columns: 4 to 7 us; with a quarter of the threads and a load at a time 20 to 32).
-constexpr int kSumColumns = 16, kSumThreads = 1024, kSumUnroll = 4;
+// 602 columns: 4 to 7 us; with a quarter of the threads and a load at a time 20 to 32).  Of rows of more than half a million columns a workgroup takes
+// several sixteens: a launch has fewer than 2^32 threads a dimension.
+constexpr int kSumColumns = 16, kSumThreads = 1024, kSumUnroll = 4, kSumWorkgroups = 1 << 16;
 
 template <typename C, typename P>
 __global__ __launch_bounds__(kSumThreads) void norm_sum_parts_kernel(const C *partial, int64_t parts, int64_t F, P *dweight, P *dbias) {
     constexpr int GROUPS = kSumThreads / kSumColumns;
     __shared__ double sums[GROUPS][kSumColumns];
     const int lane = threadIdx.x % kSumColumns, group = threadIdx.x / kSumColumns;
-    const int64_t c = (int64_t)blockIdx.x * kSumColumns + lane;
-    double sum = 0;
-    if (c < 2 * F)
-        for (int64_t k = group; k < parts; k += GROUPS * kSumUnroll) {
-            C part[kSumUnroll];
+    for (int64_t first = (int64_t)blockIdx.x * kSumColumns; first < 2 * F; first += (int64_t)gridDim.x * kSumColumns) {
+        const int64_t c = first + lane;
+        double sum = 0;
+        if (c < 2 * F)
+            for (int64_t k = group; k < parts; k += GROUPS * kSumUnroll) {
+                C part[kSumUnroll];
 #pragma unroll
-            for (int u = 0; u < kSumUnroll; ++u) part[u] = k + u * GROUPS < parts ? partial[(k + u * GROUPS) * 2 * F + c] : C(0);
+                for (int u = 0; u < kSumUnroll; ++u) part[u] = k + u * GROUPS < parts ? partial[(k + u * GROUPS) * 2 * F + c] : C(0);
 #pragma unroll
-            for (int u = 0; u < kSumUnroll; ++u) sum += (double)part[u];
+                for (int u = 0; u < kSumUnroll; ++u) sum += (double)part[u];
+            }
+        sums[group][lane] = sum;
+#pragma unroll
+        for (int half = GROUPS / 2; half > 0; half /= 2) {
+            __syncthreads();
+            if (group < half) sums[group][lane] += sums[group + half][lane];
         }
-    sums[group][lane] = sum;
-#pragma unroll
-    for (int half = GROUPS / 2; half > 0; half /= 2) {
-        __syncthreads();
-        if (group < half) sums[group][lane] += sums[group + half][lane];
+        P *to = c < F ? dweight : dbias;
+        if (group == 0 && c < 2 * F && to) to[c < F ? c : c - F] = (P)(compute_t<P>)sums[0][lane];
+        __syncthreads();  // the places are written again
     }
-    if (group != 0 || c >= 2 * F) return;
-    P *to = c < F ? dweight : dbias;
-    if (to) to[c < F ? c : c - F] = (P)(compute_t<P>)sums[0][lane];
 }
 
 template <typename T, bool RELU, bool DROP>
@@ -436,7 +439,7 @@ int norm_backward_typed(NormArgs<T> a, bool drops, int param_dtype, void *dweigh
     const int rc = drops ? (a.relu ? gradients_launch<T, true, true>(a, shape, parts, stream) : gradients_launch<T, false, true>(a, shape, parts, stream))
                          : (a.relu ? gradients_launch<T, true, false>(a, shape, parts, stream) : gradients_launch<T, false, false>(a, shape, parts, stream));
     if (rc != CGNN_OK || !sums || alone) return rc;
-    const dim3 columns((unsigned)ceil_div(2 * a.F, kSumColumns));
+    const dim3 columns((unsigned)std::min<int64_t>(ceil_div(2 * a.F, kSumColumns), kSumWorkgroups));
     if (param_dtype == CGNN_F32)
         hipLaunchKernelGGL((norm_sum_parts_kernel<C, float>), columns, dim3(kSumThreads), 0, stream, a.partial, parts, a.F,
                            static_cast<float *>(dweight), static_cast<float *>(dbias));

@@ -1,0 +1,33 @@
+"""Layer norm and dropout on the GPU at the ends of their range: sizes, sums and shapes that single steps of them are chosen by."""
+import pytest
+import torch
+
+import compressgnn_runtime as rt
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F16, BF16, F32, F64 = torch.float16, torch.bfloat16, torch.float32, torch.float64
+
+
+def normal(shape, dtype, seed):
+    """Made in the type itself: no copy of a large matrix in another."""
+    return torch.empty(shape, dtype=dtype, device=DEV).normal_(generator=torch.Generator(DEV).manual_seed(seed))
+
+
+def test_sums_of_more_columns_than_one_launch_has_threads_for():
+    """65 rows are two parts, whose sums over 2^25 + 24 columns of the weight's and the bias's gradient take workgroups of several sixteens.
+    A part's lane adds 16 rows, four of them a part, and the two parts are added in 64 bits."""
+    rows, width = 65, (1 << 25) + 24
+    x, grad = normal((rows, width), BF16, 1), normal((rows, width), BF16, 2)
+    _, stats = rt.layer_norm_forward(x, None, None, 1e-5)
+    _, dw, db = rt.layer_norm_backward(grad, x, stats, None, None)
+    assert dw.dtype == BF16 and dw.shape == db.shape == (width,)
+    mean, rstd = stats[:, :1], stats[:, 1:]
+    for first in range(0, width, 1 << 21):
+        columns = slice(first, min(width, first + (1 << 21)))
+        g, h = grad[:, columns].double(), (x[:, columns].double() - mean) * rstd
+        for got, terms in ((dw, g * h), (db, g)):
+            want = terms.sum(0)
+            off = (16 + 4 + 4) * 2.0 ** -24 * terms.abs().sum(0)  # chain, groups, and four roundings of a term
+            bound = off + 2.0 ** -8 * (want.abs() + off) + 2.0 ** -133
+            assert bool(((got[columns].double() - want).abs() <= bound).all()), first

@@ -3,7 +3,10 @@ import glob
 import os
 import re
 
+import pytest
+
 from compressgnn_amd import build
+from launches import record
 
 
 # ------------------------------------------------------------------------- sources --
@@ -27,3 +30,21 @@ def test_wide_stores_in_assembly_keep_their_registers():
                 waited = re.match(r"s_nop (\d+)$", steps[k + 1]) if k + 1 < len(steps) else None
                 assert waited and int(waited[1]) + 1 >= 2, (name, text)
     assert stores
+
+
+# ------------------------------------------------------------------------ launches --
+def _fits(launches):
+    """What HIP takes: fewer than 2^32 threads a dimension, fewer than 2^31 workgroups in the first and 2^16 in the others."""
+    for kernel, grid, block in launches:
+        for k in range(3):
+            assert 1 <= grid[k] < (1 << 31 if k == 0 else 1 << 16) and grid[k] * block[k] < 1 << 32, (kernel, grid, block)
+
+
+@pytest.mark.parametrize("dtype,width", [(3, 1 << 25), (2, (1 << 25) + 16), (0, 1 << 26), (1, 1 << 27), (3, (1 << 31) - 65537)])
+def test_sums_of_wide_parameters_fit_a_launch(tmp_path, dtype, width):
+    calls = [dict(op="gradients", rows=rows, F=width, dtype=dtype, relu=True, kept=30000) for rows in (1, 64, 65, 1000)]
+    results, _ = record(tmp_path, calls)
+    for call, (status, launches) in zip(calls, results):
+        assert status == 0 and launches[0][0][0] == "norm_long_dx_kernel", call
+        assert ("norm_sum_parts_kernel" in [kernel[0] for kernel, _, _ in launches]) == (call["rows"] > 64)
+        _fits(launches)
