@@ -12,6 +12,7 @@ struct DropoutArgs {
     int64_t rows, F, ldx;
     Drop drop;
     int64_t packs;  // of 16 bytes per row, the last ones maybe empty: as many as the row's calls of the generator serve
+    int64_t first;  // workgroup of the matrix that the launch begins with
     bool streamed;
 };
 
@@ -24,7 +25,7 @@ __global__ __launch_bounds__(kBlock) void dropout_kernel(DropoutArgs<T> a) {
     using C = compute_t<T>;
     constexpr int N = 16 / (int)sizeof(T), SHARE = kDrawn / N, PACKS = SHARE < 2 ? 2 : SHARE;
     const uint64_t offset = drop_offset(a.drop);
-    const int64_t begin = (int64_t)blockIdx.x * kBlock * PACKS, extent = (a.rows - 1) * a.ldx + a.F;
+    const int64_t begin = (a.first + blockIdx.x) * kBlock * PACKS, extent = (a.rows - 1) * a.ldx + a.F;
     const int64_t row0 = FLAT ? 0 : begin / a.packs, pack0 = begin - row0 * a.packs;
     const float inverse = 1.0f / (float)a.packs;
     int64_t row[PACKS], pack[PACKS];
@@ -92,6 +93,9 @@ __global__ __launch_bounds__(kBlock) void dropout_few_kernel(DropoutArgs<T> a) {
     }
 }
 
+// A launch has fewer than 2^32 threads a dimension: a matrix of more (some 2^33 rows of one 16-bit feature) takes several.
+constexpr int64_t kLaunched = ((int64_t)1 << 31) / kBlock;  // workgroups
+
 template <typename T>
 int dropout_launch(DropoutArgs<T> a, hipStream_t stream) {
     constexpr int N = 16 / (int)sizeof(T), SHARE = kDrawn / N, PACKS = SHARE < 2 ? 2 : SHARE;
@@ -107,12 +111,16 @@ int dropout_launch(DropoutArgs<T> a, hipStream_t stream) {
     }
     a.packs = a.drop.blocks * SHARE;
     const int64_t packs = flat ? ceil_div(a.F, N) : a.rows * a.packs, workgroups = ceil_div(packs, (int64_t)kBlock * PACKS);
-    CGNN_REQUIRE(workgroups < (int64_t)1 << 31, "cgnn_dropout: too many elements for one launch");
-    if (flat)
-        hipLaunchKernelGGL((dropout_kernel<T, true>), dim3((unsigned)workgroups), dim3(kBlock), 0, stream, a);
-    else
-        hipLaunchKernelGGL((dropout_kernel<T, false>), dim3((unsigned)workgroups), dim3(kBlock), 0, stream, a);
-    return check_launch("dropout");
+    CGNN_REQUIRE(workgroups < (int64_t)1 << 31, "cgnn_dropout: too many elements");
+    for (; a.first < workgroups; a.first += kLaunched) {
+        const dim3 grid((unsigned)std::min(workgroups - a.first, kLaunched));
+        if (flat)
+            hipLaunchKernelGGL((dropout_kernel<T, true>), grid, dim3(kBlock), 0, stream, a);
+        else
+            hipLaunchKernelGGL((dropout_kernel<T, false>), grid, dim3(kBlock), 0, stream, a);
+        if (int rc = check_launch("dropout")) return rc;
+    }
+    return CGNN_OK;
 }
 
 }  // namespace

@@ -3,6 +3,8 @@ import pytest
 import torch
 
 import compressgnn_runtime as rt
+from CompressgnnDropout import dropout
+from rows_reference import mask
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -31,3 +33,18 @@ def test_sums_of_more_columns_than_one_launch_has_threads_for():
             off = (16 + 4 + 4) * 2.0 ** -24 * terms.abs().sum(0)  # chain, groups, and four roundings of a term
             bound = off + 2.0 ** -8 * (want.abs() + off) + 2.0 ** -133
             assert bool(((got[columns].double() - want).abs() <= bound).all()), first
+
+
+def test_masks_of_more_rows_than_one_launch_has_threads_for():
+    """A column of 2^33 + 1,000: the mask of a row is that of its place in the whole matrix, in the second launch and further ones too."""
+    rows = (1 << 33) + 1000
+    out = dropout(torch.ones(rows, 1, dtype=BF16, device=DEV), 0.5, 3, 1)
+    launch = (1 << 31) // 256 * 512  # rows
+    for first in [0, (1 << 32) - 100] + [k * launch - 100 for k in range(1, 3)] + [rows - 500]:
+        kept = mask(200, 1, 0.5, 3, 1, first_row=first)
+        assert torch.equal(out[first:first + 200].cpu(), torch.from_numpy(kept).to(BF16) * 2), first
+    assert bool((out[-300:].cpu() == torch.from_numpy(mask(300, 1, 0.5, 3, 1, first_row=rows - 300)).to(BF16) * 2).all())
+    for first in range(0, rows, 1 << 31):
+        part = out[first:first + (1 << 31)].view(torch.int16)
+        share = (part == 0x4000).sum(dtype=torch.int64) + (part == 0).sum(dtype=torch.int64)  # 2 or 0
+        assert int(share) == part.numel(), first

@@ -48,3 +48,15 @@ def test_sums_of_wide_parameters_fit_a_launch(tmp_path, dtype, width):
         assert status == 0 and launches[0][0][0] == "norm_long_dx_kernel", call
         assert ("norm_sum_parts_kernel" in [kernel[0] for kernel, _, _ in launches]) == (call["rows"] > 64)
         _fits(launches)
+
+
+@pytest.mark.parametrize("rows,width,dtype", [((1 << 33) - 512, 1, 3), (1 << 33, 1, 3), ((1 << 33) + 1000, 1, 2), ((1 << 35) + 5, 1, 0), (1 << 32, 1, 1),
+                                              (1 << 33, 8, 3), ((1 << 20) + 1, 12345, 3)])
+def test_dropout_of_any_number_of_rows_fits_its_launches(tmp_path, rows, width, dtype):
+    (status, launches), = record(tmp_path, [dict(op="dropout", rows=rows, F=width, dtype=dtype, kept=30000)])[0]
+    assert status == 0 and {kernel[0] for kernel, _, _ in launches} == {"dropout_kernel"}
+    _fits(launches)
+    packs = 16 // (8 if dtype == 1 else 4 if dtype == 0 else 2)
+    lane = max(2, 8 // packs)  # packs that a lane takes
+    whole = -(-width // 8) * (8 // packs) * rows if width % 8 else width * rows // packs
+    assert sum(grid[0] for _, grid, _ in launches) == -(-whole // (256 * lane))
