@@ -222,8 +222,10 @@ int norm_launch(NormArgs<T> a, hipStream_t stream) {
     int64_t workgroups = row_workgroups(a.rows, shape, sizeof(T), false);
     a.walk = {groups, groups * workgroups, ceil_div(tiles, workgroups)};
     if (bytes >= (int64_t)1 << 30) {
-        a.walk = {groups * kLargeRounds, groups, kLargeRounds};
-        workgroups = ceil_div(tiles, kLargeRounds);
+        // more rounds where a launch, which has fewer than 2^32 threads a dimension, would not hold the workgroups
+        const int64_t rounds = std::max(kLargeRounds, ceil_div(tiles, ((int64_t)1 << 31) / shape.threads));
+        a.walk = {groups * rounds, groups, rounds};
+        workgroups = ceil_div(tiles, rounds);
     }
     a.streamed = streams(a.rows, a.F * (int64_t)sizeof(T), shape.lanes * 16, 2);
     return with_row_shape<T, false>(shape, [&](auto tag) {

@@ -60,3 +60,12 @@ def test_dropout_of_any_number_of_rows_fits_its_launches(tmp_path, rows, width, 
     lane = max(2, 8 // packs)  # packs that a lane takes
     whole = -(-width // 8) * (8 // packs) * rows if width % 8 else width * rows // packs
     assert sum(grid[0] for _, grid, _ in launches) == -(-whole // (256 * lane))
+
+
+@pytest.mark.parametrize("rows,width,dtype", [(1 << 35, 1, 2), ((1 << 35) + 77, 1, 3), ((1 << 35) - 2048, 1, 2), (1 << 36, 1, 2), (1 << 35, 9, 3), (1 << 35, 3, 0),
+                                              (1 << 29, 128, 2), (1 << 26, 1200, 3), (1 << 24, 8000, 0), (1 << 40, 1, 1)])
+def test_norms_of_any_number_of_rows_fit_a_launch(tmp_path, rows, width, dtype):
+    calls = [dict(op=op, rows=rows, F=width, dtype=dtype, relu=True, kept=30000) for op in ("norm", "gradients")]
+    for status, launches in record(tmp_path, calls)[0]:
+        assert status == 0
+        _fits(launches)
