@@ -48,3 +48,27 @@ def test_masks_of_more_rows_than_one_launch_has_threads_for():
         part = out[first:first + (1 << 31)].view(torch.int16)
         share = (part == 0x4000).sum(dtype=torch.int64) + (part == 0).sum(dtype=torch.int64)  # 2 or 0
         assert int(share) == part.numel(), first
+
+
+@pytest.mark.parametrize("dtype,width", [(F32, 20_000_003), (BF16, 24_000_001), (F16, 9000), (F32, 8200)])
+def test_sums_along_wide_rows_do_not_lose_with_the_width(dtype, width):
+    """A gradient that is one number everywhere: its mean takes all of it away again, so what a chain of float additions along the row loses
+    stays in dx.  Sums of a pack or two in float (16 additions at most), the rest in 64 bits: a bound without the width in it."""
+    rows = 2
+    x, g = normal((rows, width), dtype, 1), torch.full((rows, width), 0.1, dtype=dtype, device=DEV)
+    g[1] *= 0.25
+    _, stats = rt.layer_norm_forward(x, None, None, 1e-5)
+    dx, _, _ = rt.layer_norm_backward(g, x, stats, None, None)
+    G = g.double()
+    X = x.double()
+    mean = X.mean(1, keepdim=True)
+    rstd = 1 / torch.sqrt(((X - mean) ** 2).mean(1, keepdim=True) + 1e-5)
+    h = (X - mean) * rstd
+    m1, m2, c1, c2 = G.mean(1, keepdim=True), (G * h).abs().mean(1, keepdim=True), G.mean(1, keepdim=True), (G * h).mean(1, keepdim=True)
+    want = rstd * (G - c1 - h * c2)
+    u = 2.0 ** -24
+    # a value takes a handful of roundings, a sum 16 and a few more; 64-bit sums of 20 million terms in lanes of 20,000 lose 2^-36 at most
+    off = rstd * (8 * u * (G + m1 + h.abs() * m2) + 20 * u * (m1 + h.abs() * m2)) + 2.0 ** -36 * rstd * (m1 + h.abs() * m2)
+    bound = off + torch.finfo(dtype).eps / 2 * (want.abs() + off) + 2.0 ** -24 * (dtype == F16) + 2.0 ** -133
+    over = (dx.double() - want).abs() - bound
+    assert float(over.max()) <= 0, (float((dx.double() - want).abs().max()), float(bound.min()))
