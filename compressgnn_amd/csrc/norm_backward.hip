@@ -8,12 +8,13 @@
 namespace cgnn {
 namespace {
 
-constexpr int kLongRows = 64;   // rows longer than the registers: rows per part of the parameters' sums, at least
-constexpr int kLongParts = 512;
-constexpr int kLanes = 64;      // ... lanes side by side, a pack each
-constexpr int64_t kChain = 1024;  // other rows: as many of them at most are added up one after the other by a lane, in float
+constexpr int64_t kChain = 1024;  // rows at most that a lane adds up one after the other, in float
+constexpr int kLongRows = 64;     // rows longer than the registers: rows per part of the parameters' sums, at least
+constexpr int kLongParts = 512;   // ... parts, as long as no lane's chain grows too long for that
+constexpr int kLanes = 64;        // ... lanes side by side, a pack each
+constexpr int kLongGroups = kBlock / kLanes;
 
-int64_t long_rows(int64_t rows) { return std::max<int64_t>(kLongRows, ceil_div(rows, kLongParts)); }
+int64_t long_rows(int64_t rows) { return std::min(std::max<int64_t>(kLongRows, ceil_div(rows, kLongParts)), kLongGroups * kChain); }
 
 // Workgroups of norm_gradients_kernel, each of which leaves a part of the parameters' sums.  A part is two rows of floats: it is to stand for
 // sixteen rows or more (4,096 rows of 4,096 float16 features: 32 us with 256 parts, 35 with 512), if half the chip is not to be idle for that.
@@ -271,7 +272,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_dx_kernel(NormArgs<T> 
 template <typename T, bool RELU, bool DROP>
 __global__ __launch_bounds__(kBlock) void norm_long_parts_kernel(NormArgs<T> a, int64_t part) {
     using C = compute_t<T>;
-    constexpr int N = 16 / (int)sizeof(T), GROUPS = kBlock / kLanes;
+    constexpr int N = 16 / (int)sizeof(T), GROUPS = kLongGroups;
     __shared__ C sums[GROUPS][2][N][kLanes];
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
     const int64_t extent_x = (a.rows - 1) * a.ldx + a.F, extent_g = (a.rows - 1) * a.ldg + a.F;

@@ -69,3 +69,18 @@ def test_norms_of_any_number_of_rows_fit_a_launch(tmp_path, rows, width, dtype):
     for status, launches in record(tmp_path, calls)[0]:
         assert status == 0
         _fits(launches)
+
+
+@pytest.mark.parametrize("dtype", range(4))
+def test_parts_keep_a_lanes_chain_short(tmp_path, dtype):
+    """The parameters' sums are added in float down the rows of a part and in 64 bits from part to part: no lane adds more than 1,024 rows."""
+    calls = [dict(op="gradients", rows=rows, F=width, dtype=dtype) for width in (1, 40, 1000, 8193, 20001)
+             for rows in (5, 1000, 100003, (1 << 21) + 5, 1 << 24, (1 << 28) - 1) if rows * width < 1 << 38]
+    for call, (status, launches) in zip(calls, record(tmp_path, calls)[0]):
+        assert status == 0
+        _fits(launches)
+        for (name, values), grid, block in launches:
+            if name == "norm_gradients_kernel":
+                assert -(-call["rows"] // (grid[0] * (block[0] // values[1]))) <= 1024, call
+            if name == "norm_long_parts_kernel":
+                assert -(-call["rows"] // grid[1]) <= 4 * 1024, call
