@@ -51,25 +51,28 @@ __global__ __launch_bounds__(THREADS) void norm_rows_kernel(NormArgs<T> a) {
         Pack<T, N> x[K];
         const T first = next_first;
         row_arrived<T, LANES, K>(next, a.x, r * a.ldx, extent, lane, F, x);
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-            if ((lane + k * LANES) * N + N > F)  // what lies behind the row's end adds nothing to its sums
-#pragma unroll
-                for (int i = 0; i < N; ++i)
-                    if ((lane + k * LANES) * N + i >= F) x[k].v[i] = first;
         ask(r + step < end ? r + step : r);
-        const double pivot = (double)first;
-        double sum = 0, squares = 0;
+        auto about = [&](T pivot) {
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+            for (int k = 0; k < K; ++k)
+                if ((lane + k * LANES) * N + N > F)  // what lies behind the row's end adds nothing to its sums
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const double d = (double)x[k].v[i] - pivot;
-                sum += d;
-                squares = __builtin_fma(d, d, squares);
-            }
-        row_sums<LANES, THREADS>(sum, squares, scratch, odd);
-        const Moments m = moments(pivot, sum, squares, a.inverse_F);
+                    for (int i = 0; i < N; ++i)
+                        if ((lane + k * LANES) * N + i >= F) x[k].v[i] = pivot;
+            double sum = 0, squares = 0;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const double d = (double)x[k].v[i] - (double)pivot;
+                    sum += d;
+                    squares = __builtin_fma(d, d, squares);
+                }
+            row_sums<LANES, THREADS>(sum, squares, scratch, odd);
+            return moments((double)pivot, sum, squares, a.inverse_F);
+        };
+        Moments m = about(first);
+        if constexpr (sizeof(T) == 8) m = about(m.mean);
         const Centre<C> centre(m.mean, reciprocal_root(m.variance + a.eps));
         Pack<T, N> y[K];
         Draws drawn[K];
@@ -97,7 +100,7 @@ __global__ __launch_bounds__(THREADS) void norm_rows_kernel(NormArgs<T> a) {
     }
 }
 
-// Longer rows: a workgroup a row, which reads it twice, kLongPacks packs a lane at a time.  Bound by the latency of the two
+// Longer rows: a workgroup a row, which reads it twice (float64: three times), kLongPacks packs a lane at a time.  Bound by the latency of the two
 // readings, one workgroup a compute unit (3,000 rows of 20,000 float32 features: 208 us, 2.3 TB/s; a pack at a time 299).
 template <typename T, bool RELU, bool DROP>
 __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs<T> a) {
@@ -110,30 +113,32 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs<T> a) 
     const int64_t extent = (a.rows - 1) * a.ldx + a.F;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const int64_t at = r * a.ldx;
-        const T first = a.x[at];
-        const double pivot = (double)first;
-        double sum = 0, squares = 0;
         words_t asked[kLongPacks];
         auto ask = [&](int64_t j0) {
 #pragma unroll
             for (int k = 0; k < kLongPacks; ++k) asked[k] = ask_within<T>(a.x, at + std::min(j0 + k * kStride, a.F - 1), extent);
         };
-        for (int64_t j0 = (int64_t)threadIdx.x * N; j0 < a.F; j0 += kLongPacks * kStride) {
-            ask(j0);
+        auto about = [&](T pivot) {
+            double sum = 0, squares = 0;
+            for (int64_t j0 = (int64_t)threadIdx.x * N; j0 < a.F; j0 += kLongPacks * kStride) {
+                ask(j0);
 #pragma unroll
-            for (int k = 0; k < kLongPacks; ++k) {
-                const int64_t j = j0 + k * kStride;
-                const auto x = settled<T>(asked[k], a.x, at + std::min(j, a.F - 1), extent);
+                for (int k = 0; k < kLongPacks; ++k) {
+                    const int64_t j = j0 + k * kStride;
+                    const auto x = settled<T>(asked[k], a.x, at + std::min(j, a.F - 1), extent);
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const double d = j + i < a.F ? (double)x.v[i] - pivot : 0.0;
-                    sum += d;
-                    squares = __builtin_fma(d, d, squares);
+                    for (int i = 0; i < N; ++i) {
+                        const double d = j + i < a.F ? (double)x.v[i] - (double)pivot : 0.0;
+                        sum += d;
+                        squares = __builtin_fma(d, d, squares);
+                    }
                 }
             }
-        }
-        row_sums<kLongThreads, kLongThreads>(sum, squares, scratch, odd);
-        const Moments m = moments(pivot, sum, squares, a.inverse_F);
+            row_sums<kLongThreads, kLongThreads>(sum, squares, scratch, odd);
+            return moments((double)pivot, sum, squares, a.inverse_F);
+        };
+        Moments m = about(a.x[at]);
+        if constexpr (sizeof(T) == 8) m = about(m.mean);
         const Centre<C> centre(m.mean, reciprocal_root(m.variance + a.eps));
         if (a.stats && threadIdx.x == 0) {
             a.stats[2 * r] = centre.mean;
@@ -177,13 +182,17 @@ __global__ __launch_bounds__(kWave) void norm_few_kernel(NormArgs<T> a) {
     const int64_t r = threadIdx.x;
     if (r >= a.rows) return;
     const T *x = a.x + r * a.ldx;
-    double sum = 0, squares = 0;
-    for (int64_t j = 0; j < a.F; ++j) {
-        const double d = (double)x[j] - (double)x[0];
-        sum += d;
-        squares = __builtin_fma(d, d, squares);
-    }
-    const Moments m = moments((double)x[0], sum, squares, a.inverse_F);
+    auto about = [&](T pivot) {
+        double sum = 0, squares = 0;
+        for (int64_t j = 0; j < a.F; ++j) {
+            const double d = (double)x[j] - (double)pivot;
+            sum += d;
+            squares = __builtin_fma(d, d, squares);
+        }
+        return moments((double)pivot, sum, squares, a.inverse_F);
+    };
+    Moments m = about(x[0]);
+    if constexpr (sizeof(T) == 8) m = about(m.mean);
     const Centre<C> centre(m.mean, reciprocal_root(m.variance + a.eps));
     if (a.stats) {
         a.stats[2 * r] = centre.mean;

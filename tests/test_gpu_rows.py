@@ -1,4 +1,5 @@
 """Layer norm and dropout on the GPU at the ends of their range: sizes, sums and shapes that single steps of them are chosen by."""
+import numpy as np
 import pytest
 import torch
 
@@ -72,3 +73,22 @@ def test_sums_along_wide_rows_do_not_lose_with_the_width(dtype, width):
     bound = off + torch.finfo(dtype).eps / 2 * (want.abs() + off) + 2.0 ** -24 * (dtype == F16) + 2.0 ** -133
     over = (dx.double() - want).abs() - bound
     assert float(over.max()) <= 0, (float((dx.double() - want).abs().max()), float(bound.min()))
+
+
+@pytest.mark.parametrize("width", [3, 33, 100, 257, 1024, 1500, 4100, 8192, 20001])
+@pytest.mark.parametrize("rows", [2, 2000])
+def test_float64_statistics_with_an_outlier_in_front(rows, width):
+    """The first element a million deviations of the others off: differences to it alone would leave log2(width) bits less of the variance.
+    Lanes add up to width / 64 terms (longer rows: width / 1,024 and 16 waves' sums), then six steps across lanes; a square or a difference
+    has two roundings."""
+    x = normal((rows, width), F64, 1)
+    x[:, 0] = 1e6
+    _, stats = rt.layer_norm_forward(x, None, None, 0.0)
+    exact = x[:2].cpu().numpy().astype(np.longdouble)  # 64 bits of mantissa
+    mean = exact.mean(1, keepdims=True)
+    rstd = 1 / np.sqrt(((exact - mean) ** 2).mean(1))
+    got = stats[:2].cpu().numpy()
+    steps = 4 + 24 + min(width, 4096) / 64 + width / 1024
+    assert (np.abs(got[:, 0] - mean[:, 0]) <= steps * 2.0 ** -53 * np.abs(exact).mean(1)).all()
+    assert (np.abs(got[:, 1] / rstd - 1) <= steps * 2.0 ** -53).all(), np.abs(got[:, 1] / rstd - 1) * 2.0 ** 53
+    assert bool((stats[:, 1] - stats[0, 1]).abs().max() < 1e-3 * stats[0, 1])
