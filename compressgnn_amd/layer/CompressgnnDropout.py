@@ -44,7 +44,8 @@ class Masks:
     Calls under a stream capture are numbered on the device, by a counter that the captured work itself
     counts up, and lie in a range of their own; the module has to be on the device of the rows before.  A copy of a module
     draws the masks that the module draws.  A forward pass computed again in a backward one (activation checkpointing) would draw
-    other masks than the first time and is refused: there the functions, whose masks have names, serve."""
+    other masks than the first time and is refused, and so is one under a trace (torch.jit.trace), which would hold one call's number and
+    drop the same elements in every run: there the functions, whose masks have names, serve."""
 
     CAPTURED = 1 << 62  # offsets of captured calls begin here
 
@@ -59,6 +60,9 @@ class Masks:
         if _native.in_backward():
             raise RuntimeError("a call within a backward pass would draw another mask than the forward pass did; call dropout or "
                                "norm_act_dropout with a seed and an offset where activations are computed again")
+        if torch.jit.is_tracing():
+            raise RuntimeError("a trace would draw the mask of this one call in every run; trace the module in eval mode, or call dropout or "
+                               "norm_act_dropout with a seed, an offset and a counter on the device")
         if x.is_cuda and torch.cuda.is_current_stream_capturing():
             if self.replays.device != x.device:
                 raise RuntimeError("the module is on %s and x on %s: move it there before the capture" % (self.replays.device, x.device))

@@ -4,7 +4,8 @@ import pytest
 import torch
 
 import compressgnn_runtime as rt
-from CompressgnnDropout import dropout
+from CompressgnnDropout import Compressgnn_Dropout, dropout
+from CompressgnnNorm import Compressgnn_LayerNorm
 from rows_reference import mask
 
 pytestmark = pytest.mark.gpu
@@ -92,3 +93,20 @@ def test_float64_statistics_with_an_outlier_in_front(rows, width):
     assert (np.abs(got[:, 0] - mean[:, 0]) <= steps * 2.0 ** -53 * np.abs(exact).mean(1)).all()
     assert (np.abs(got[:, 1] / rstd - 1) <= steps * 2.0 ** -53).all(), np.abs(got[:, 1] / rstd - 1) * 2.0 ** 53
     assert bool((stats[:, 1] - stats[0, 1]).abs().max() < 1e-3 * stats[0, 1])
+
+
+# ------------------------------------------------------------------------- modules --
+def test_a_module_in_training_is_not_traced():
+    x = normal((20, 12), F32, 1)
+    for module in (Compressgnn_Dropout(0.5).to(DEV), Compressgnn_LayerNorm(12, activation="relu", p=0.5).to(DEV)):
+        with pytest.raises(RuntimeError, match="a trace would draw"):
+            torch.jit.trace(module, (x,), check_trace=False)
+        module.eval()
+        traced = torch.jit.trace(module, (x,), check_trace=False)
+        assert torch.equal(traced(2 * x), module(2 * x))
+    # what the message names instead: masks that a counter on the device tells apart
+    counter = torch.zeros(1, dtype=torch.int64, device=DEV)
+    traced = torch.jit.trace(lambda x, counter: dropout(x, 0.5, 3, 0, counter), (x, counter), check_trace=False)
+    for n in range(3):
+        counter.fill_(n)
+        assert torch.equal(traced(x, counter), dropout(x, 0.5, 3, n))

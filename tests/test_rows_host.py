@@ -4,8 +4,11 @@ import os
 import re
 
 import pytest
+import torch
 
 from compressgnn_amd import build
+from CompressgnnDropout import Compressgnn_Dropout
+from CompressgnnNorm import Compressgnn_LayerNorm
 from launches import record
 
 
@@ -84,3 +87,20 @@ def test_parts_keep_a_lanes_chain_short(tmp_path, dtype):
                 assert -(-call["rows"] // (grid[0] * (block[0] // values[1]))) <= 1024, call
             if name == "norm_long_parts_kernel":
                 assert -(-call["rows"] // grid[1]) <= 4 * 1024, call
+
+
+# ------------------------------------------------------------------------- modules --
+@pytest.mark.parametrize("module", [Compressgnn_Dropout(0.5, seed=1), Compressgnn_LayerNorm(4, p=0.5, seed=1)])
+def test_a_module_draws_no_mask_under_a_trace(module):
+    """The number of the call would be a constant of the trace, and every run of it drop the same elements."""
+    class Masked(torch.nn.Module):
+        def forward(self, x):
+            return x * float(module._next_mask(x)[1])
+
+    with pytest.raises(RuntimeError, match="a trace would draw"):
+        torch.jit.trace(Masked(), (torch.ones(3, 4),), check_trace=False)
+    assert module.calls == 0
+    # in eval mode nothing is drawn, and a trace of the whole module holds what it computes
+    drop = Compressgnn_Dropout(0.5).eval()
+    x = torch.ones(3, 4)
+    assert torch.equal(torch.jit.trace(drop, (x,), check_trace=False)(x * 2), x * 2)
