@@ -5,6 +5,8 @@ position of an element, in the forward pass and again in the gradient.  The shar
 nearest 65,536th and the scale is its reciprocal.  Rows are the last dimension; the mask of an element depends on its row and
 its column, not on the type or on strides.
 """
+import copy
+
 import _paths  # noqa: F401
 import torch
 from torch.autograd.function import once_differentiable
@@ -38,22 +40,34 @@ def dropout(x, p, seed, offset=0, counter=None):
     return _Dropped.apply(x, p, seed, offset, counter) if out is None else out
 
 
+def _fresh_seed():
+    """Of torch's own generator, where none is given: torch.manual_seed fixes it, and no two modules share masks."""
+    return int(torch.randint(1 << 62, (1,)))
+
+
 class Masks:
     """The masks of a module, one after the other: each is named by the module's seed and the number of the call.
 
     Calls under a stream capture are numbered on the device, by a counter that the captured work itself
-    counts up, and lie in a range of their own; the module has to be on the device of the rows before.  A copy of a module
-    draws the masks that the module draws.  A forward pass computed again in a backward one (activation checkpointing) would draw
+    counts up, and lie in a range of their own; the module has to be on the device of the rows before.  A deep copy of a
+    module, as layers are stacked with, is a module of its own and gets a seed of its own, of torch's generator; the state dict carries the
+    seed and the place from one module to another.  A forward pass computed again in a backward one (activation checkpointing) would draw
     other masks than the first time and is refused, and so is one under a trace (torch.jit.trace), which would hold one call's number and
     drop the same elements in every run: there the functions, whose masks have names, serve."""
 
     CAPTURED = 1 << 62  # offsets of captured calls begin here
 
     def _init_masks(self, seed):
-        # of torch's own generator where none is given: torch.manual_seed fixes it, and no two modules share masks
-        self.seed = int(torch.randint(1 << 62, (1,))) if seed is None else int(seed)
+        self.seed = _fresh_seed() if seed is None else int(seed)
         self.calls = 0
         self.register_buffer('replays', torch.zeros(1, dtype=torch.int64))
+
+    def __deepcopy__(self, memo):
+        twin = type(self).__new__(type(self))
+        memo[id(self)] = twin
+        twin.__dict__.update(copy.deepcopy(self.__dict__, memo))
+        twin.seed = _fresh_seed()
+        return twin
 
     def _next_mask(self, x):
         """(seed, offset, counter) of a call on x"""

@@ -1,6 +1,8 @@
 """The row-wise operators as far as the host alone shows them: their sources, launches, modules.  No GPU needed."""
+import copy
 import glob
 import os
+import pickle
 import re
 
 import pytest
@@ -104,3 +106,34 @@ def test_a_module_draws_no_mask_under_a_trace(module):
     drop = Compressgnn_Dropout(0.5).eval()
     x = torch.ones(3, 4)
     assert torch.equal(torch.jit.trace(drop, (x,), check_trace=False)(x * 2), x * 2)
+
+
+def test_deep_copies_draw_masks_of_their_own():
+    """As layers are stacked: one is made and copied, and no two of them may drop the same elements."""
+    layer = torch.nn.Sequential(torch.nn.Linear(4, 4), Compressgnn_LayerNorm(4, activation="relu", p=0.5, seed=5), Compressgnn_Dropout(0.3))
+    layer[1].weight.data.fill_(2.0)
+    layer[1].calls, layer[1].tied = 7, layer[1].weight
+    layer[1].replays.fill_(3)
+    before = layer[1].seed
+    stack = [copy.deepcopy(layer) for _ in range(6)] + [layer]
+    assert layer[1].seed == before
+    for k in (1, 2):
+        assert len({layers[k].seed for layers in stack}) == len(stack)
+    for layers in stack[:-1]:
+        norm = layers[1]
+        assert type(norm) is Compressgnn_LayerNorm and norm.p == 0.5 and norm.activation == "relu" and norm.calls == 7
+        assert torch.equal(norm.weight, layer[1].weight) and norm.weight is not layer[1].weight and norm.tied is norm.weight
+        assert isinstance(norm.weight, torch.nn.Parameter) and norm.replays.tolist() == [3] and norm.replays is not layer[1].replays
+        assert [name for name, _ in layers.named_parameters()] == [name for name, _ in layer.named_parameters()]
+    torch.manual_seed(11)
+    seeds = [copy.deepcopy(layer[2]).seed for _ in range(2)]
+    torch.manual_seed(11)
+    assert [copy.deepcopy(layer[2]).seed for _ in range(2)] == seeds and seeds[0] != seeds[1]
+    twice = copy.deepcopy([layer[2], layer[2]])  # one module twice stays one
+    assert twice[0] is twice[1]
+    # the state dict and a pickle carry the place in the masks
+    other = copy.deepcopy(layer)
+    other.load_state_dict(layer.state_dict())
+    assert (other[1].seed, other[1].calls) == (before, 7) and other[2].seed == layer[2].seed
+    same = pickle.loads(pickle.dumps(layer))
+    assert (same[1].seed, same[1].calls, same[2].seed) == (before, 7, layer[2].seed)
