@@ -6,6 +6,7 @@ nearest 65,536th and the scale is its reciprocal.  Rows are the last dimension; 
 its column, not on the type or on strides.
 """
 import copy
+import threading
 
 import _paths  # noqa: F401
 import torch
@@ -43,6 +44,9 @@ def dropout(x, p, seed, offset=0, counter=None):
 def _fresh_seed():
     """Of torch's own generator, where none is given: torch.manual_seed fixes it, and no two modules share masks."""
     return int(torch.randint(1 << 62, (1,)))
+
+
+_numbering = threading.Lock()  # no two calls get one number, whatever threads they come from
 
 
 class Masks:
@@ -83,8 +87,10 @@ class Masks:
             counter = self.replays + 0
             self.replays += 1
             return self.seed, self.CAPTURED, counter
-        self.calls += 1
-        return self.seed, self.calls - 1, None
+        with _numbering:
+            number = self.calls
+            self.calls = number + 1
+        return self.seed, number, None
 
     def get_extra_state(self):
         return torch.tensor([self.seed, self.calls], dtype=torch.int64)

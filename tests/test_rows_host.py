@@ -4,6 +4,7 @@ import glob
 import os
 import pickle
 import re
+import threading
 
 import pytest
 import torch
@@ -137,3 +138,28 @@ def test_deep_copies_draw_masks_of_their_own():
     assert (other[1].seed, other[1].calls) == (before, 7) and other[2].seed == layer[2].seed
     same = pickle.loads(pickle.dumps(layer))
     assert (same[1].seed, same[1].calls, same[2].seed) == (before, 7, layer[2].seed)
+
+
+def test_calls_from_two_threads_get_two_numbers():
+    """A second call that comes while the first is between reading the count and writing it: forced, not hoped for."""
+    numbers = {}
+
+    class Slow(Compressgnn_Dropout):
+        @property
+        def calls(self):
+            return self.__dict__["_calls"]
+
+        @calls.setter
+        def calls(self, value):
+            self.__dict__["_calls"] = value
+            if value == 1 and "second" not in numbers:
+                numbers["second"] = None
+                late.start()
+                late.join(0.5)  # where calls wait for each other it comes to nothing before this one is through
+
+    module = Slow(0.5, seed=3)
+    x = torch.zeros(2, 2)
+    late = threading.Thread(target=lambda: numbers.update(second=module._next_mask(x)[1]))
+    first = module._next_mask(x)[1]
+    late.join(30)
+    assert sorted([first, numbers["second"]]) == [0, 1] and module.calls == 2
