@@ -98,6 +98,13 @@ class Masks:
     def set_extra_state(self, state):
         self.seed, self.calls = (int(v) for v in state)
 
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        """A state dict without a place in the masks at all is that of a model with torch's modules: the place stays as it is."""
+        missing = []
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing, unexpected_keys, error_msgs)
+        place = {prefix + "replays", prefix + "_extra_state"}
+        missing_keys += [key for key in missing if key not in place or not place.isdisjoint(state_dict)]
+
 
 class Compressgnn_Dropout(Masks, torch.nn.Module):
     """dropout(x, p) in training, x itself otherwise.  seed: fixes the masks; its own and the numbers of calls so far, captured

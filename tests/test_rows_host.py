@@ -163,3 +163,30 @@ def test_calls_from_two_threads_get_two_numbers():
     first = module._next_mask(x)[1]
     late.join(30)
     assert sorted([first, numbers["second"]]) == [0, 1] and module.calls == 2
+
+
+def test_state_dicts_of_torchs_modules_are_loaded():
+    """A model that had torch's LayerNorm and Dropout in these places: its parameters are there, a place in masks is not."""
+    theirs = torch.nn.Sequential(torch.nn.Linear(3, 4), torch.nn.LayerNorm(4), torch.nn.Dropout(0.5))
+    torch.nn.init.normal_(theirs[1].weight)
+    for p in (0.0, 0.5):
+        ours = torch.nn.Sequential(torch.nn.Linear(3, 4), Compressgnn_LayerNorm(4, p=p, seed=5), Compressgnn_Dropout(0.5, seed=6))
+        ours[1].calls = 2
+        ours[2].replays.fill_(4)
+        done = ours.load_state_dict(theirs.state_dict())
+        assert not done.missing_keys and not done.unexpected_keys
+        assert torch.equal(ours[1].weight, theirs[1].weight) and torch.equal(ours[1].bias, theirs[1].bias)
+        assert (ours[1].seed, ours[1].calls, ours[2].seed, ours[2].replays.tolist()) == (5, 2, 6, [4])
+    # half a place, and a parameter that is not there, are still missed
+    for k, lost in ((1, "1.replays"), (1, "1._extra_state"), (2, "2.replays"), (1, "1.weight"), (1, "1.bias")):
+        state = ours.state_dict()
+        del state[lost]
+        with pytest.raises(RuntimeError, match=re.escape(lost)):
+            ours.load_state_dict(state)
+        assert ours.load_state_dict(state, strict=False).missing_keys == [lost]
+    state = theirs.state_dict()
+    del state["1.bias"]
+    with pytest.raises(RuntimeError, match="1.bias"):
+        ours.load_state_dict(state)
+    with pytest.raises(RuntimeError, match="Unexpected"):
+        ours.load_state_dict(dict(theirs.state_dict(), **{"1.more": torch.zeros(1)}))
