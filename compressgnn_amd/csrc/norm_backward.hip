@@ -431,7 +431,7 @@ int gradients_launch(const NormArgs<T> &a, const RowShape &shape, int64_t parts,
 }
 
 template <typename T>
-int norm_backward_typed(NormArgs<T> a, bool drops, int param_dtype, void *dweight, void *dbias, hipStream_t stream) {
+int norm_backward_typed(NormArgs<T> a, bool drops, void *dweight, void *dbias, hipStream_t stream) {
     using C = compute_t<T>;
     const RowShape shape = row_shape(a.rows, a.F, sizeof(T), true);
     const int64_t parts = parts_of(a.rows, shape, sizeof(T));
@@ -446,13 +446,15 @@ int norm_backward_typed(NormArgs<T> a, bool drops, int param_dtype, void *dweigh
                          : (a.relu ? gradients_launch<T, true, false>(a, shape, parts, stream) : gradients_launch<T, false, false>(a, shape, parts, stream));
     if (rc != CGNN_OK || !sums || alone) return rc;
     const dim3 columns((unsigned)std::min<int64_t>(ceil_div(2 * a.F, kSumColumns), kSumWorkgroups));
-    if (param_dtype == CGNN_F32)
-        hipLaunchKernelGGL((norm_sum_parts_kernel<C, float>), columns, dim3(kSumThreads), 0, stream, a.partial, parts, a.F,
-                           static_cast<float *>(dweight), static_cast<float *>(dbias));
-    else
-        hipLaunchKernelGGL((norm_sum_parts_kernel<C, T>), columns, dim3(kSumThreads), 0, stream, a.partial, parts, a.F,
-                           static_cast<T *>(dweight), static_cast<T *>(dbias));
-    return check_launch("layer_norm_backward");
+    auto add = [&](auto tag) {
+        using P = typename decltype(tag)::type;
+        hipLaunchKernelGGL((norm_sum_parts_kernel<C, P>), columns, dim3(kSumThreads), 0, stream, a.partial, parts, a.F, static_cast<P *>(dweight),
+                           static_cast<P *>(dbias));
+        return check_launch("layer_norm_backward");
+    };
+    if constexpr (sizeof(T) == 2)
+        if (a.weight.wide) return add(TypeTag<float>());
+    return add(TypeTag<T>());
 }
 
 }  // namespace
@@ -498,6 +500,6 @@ extern "C" int cgnn_layer_norm_backward(int64_t rows, int64_t F, int dtype, int 
         a.rows = rows;
         a.F = F;
         a.inverse_F = 1.0 / (double)F;
-        return norm_backward_typed<T>(a, a.drop.kept < kAllKept, param_dtype, dweight, dbias, stream);
+        return norm_backward_typed<T>(a, a.drop.kept < kAllKept, dweight, dbias, stream);
     });
 }

@@ -687,14 +687,14 @@ int with_row_shape(const RowShape &s, F &&run) {
             if constexpr (!GRADIENT)
                 if (s.packs > 3) return s.packs == 4 ? run(ShapeTag<64, 4, 256>()) : run(ShapeTag<64, 5, 256>());
             return s.packs == 2 ? run(ShapeTag<64, 2, 256>()) : run(ShapeTag<64, 3, 256>());
-        case 128:
-            if constexpr (!GRADIENT) return s.packs == 1 ? run(ShapeTag<128, 1, 128>()) : run(ShapeTag<128, 3, 128>());
         case 256:
             if (s.packs == 1) return run(ShapeTag<256, 1, 256>());
             return s.packs == 2 ? run(ShapeTag<256, 2, 256>()) : run(ShapeTag<256, 3, 256>());
-        default:
-            if constexpr (!GRADIENT)
+        default:  // 512, and 128 in the forward pass
+            if constexpr (!GRADIENT) {
+                if (s.lanes == 128) return s.packs == 1 ? run(ShapeTag<128, 1, 128>()) : run(ShapeTag<128, 3, 128>());
                 if (s.packs == 1) return run(ShapeTag<512, 1, 512>());
+            }
             if constexpr (!GRADIENT || sizeof(T) > 2)
                 if (s.packs > 2) return s.packs == 3 ? run(ShapeTag<512, 3, 512>()) : run(ShapeTag<512, 4, 512>());
             return run(ShapeTag<512, 2, 512>());

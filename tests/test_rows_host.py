@@ -190,3 +190,12 @@ def test_state_dicts_of_torchs_modules_are_loaded():
         ours.load_state_dict(state)
     with pytest.raises(RuntimeError, match="Unexpected"):
         ours.load_state_dict(dict(theirs.state_dict(), **{"1.more": torch.zeros(1)}))
+
+
+# -------------------------------------------------------------------------- shapes --
+def test_no_sum_of_parts_is_built_that_no_call_takes(tmp_path):
+    calls = [dict(op="gradients", rows=100000, F=64, dtype=dtype, param=param) for dtype, param in ((0, 0), (1, 1), (2, 2), (2, 0), (3, 3), (3, 0))]
+    results, kernels = record(tmp_path, calls)
+    reached = {kernel for _, launches in results for kernel, _, _ in launches}
+    built = {kernel for kernel in kernels if kernel[0] == "norm_sum_parts_kernel"}
+    assert built <= reached, built - reached
