@@ -5,8 +5,9 @@ import torch
 
 import compressgnn_runtime as rt
 from CompressgnnDropout import Compressgnn_Dropout, dropout
-from CompressgnnNorm import Compressgnn_LayerNorm
-from rows_reference import mask
+from CompressgnnNorm import Compressgnn_LayerNorm, norm_act_dropout
+from row_shapes import SPREAD, many
+from rows_reference import SMALLEST, UNIT, factors, mask
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -110,3 +111,49 @@ def test_a_module_in_training_is_not_traced():
     for n in range(3):
         counter.fill_(n)
         assert torch.equal(traced(x, counter), dropout(x, 0.5, 3, n))
+
+
+# -------------------------------------------------------------------------- shapes --
+def check(got, want, off, dtype, what):
+    """Within `off` of the formula, and half a step of the type that it is rounded to."""
+    bound = off + UNIT[dtype] * (want.abs() + off) + SMALLEST[dtype]
+    over = (got.double() - want).abs() - bound
+    assert got.dtype == dtype and got.shape == want.shape and bool(torch.isfinite(got).all()), what
+    assert float(over.max()) <= 0, (what, float(over.max()), int((over > 0).sum()))
+
+
+@pytest.mark.parametrize("dtype,params", [(F32, F32), (F64, F64), (F16, F16), (F16, F32), (BF16, BF16), (BF16, F32)])
+@pytest.mark.parametrize("number", range(len(SPREAD)), ids=["%dx%d" % shape for shape in SPREAD])
+def test_rows_of_several_packs_a_lane_match_the_formulas(dtype, params, number):
+    """Outputs and gradients of matrices with more rows than the chip holds at a pack a lane, by formulas in 64 bits on the device and the bounds
+    of rows_reference.Reference; masks from the host's generator."""
+    for _, rows, width in many(dtype)[2 * number:2 * number + 2]:
+        x = normal((rows, width), F32, width).mul_(0.5 + torch.rand(rows, 1, device=DEV, generator=torch.Generator(DEV).manual_seed(5))).add_(0.3).to(dtype)
+        grad = normal((rows, width), dtype, 7)
+        w, b = (1 + 0.3 * normal((width,), F32, 3)).to(params), (0.2 * normal((width,), F32, 4)).to(params)
+        X, W, B, u = x.double(), w.double(), b.double(), 2.0 ** -53 if dtype == F64 else 2.0 ** -24
+        mean = X.mean(1, keepdim=True)
+        rstd = 1 / torch.sqrt(((X - mean) ** 2).mean(1, keepdim=True) + 1e-5)
+        h = (X - mean) * rstd
+        h_off = (width + 16) * 2.0 ** -53 * (2 * rstd * X.abs().mean(1, keepdim=True) + 2 * h.abs())
+        pre = h * W + B
+        assert float(pre.abs().min()) > 1e-12  # which side of zero the formula is on is no matter of rounding
+        for relu, p in [(False, 0.0), (True, 0.0), (False, 0.3), (True, 0.5)]:
+            what = (rows, width, relu, p)
+            factor = torch.from_numpy(factors(rows, width, p, 21, 2)).to(DEV) if p else torch.ones((), dtype=F64, device=DEV)
+            leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+            out = norm_act_dropout(*leaves, 1e-5, "relu" if relu else None, p, 21, 2)
+            dx, dw, db = torch.autograd.grad(out, leaves, grad)
+            gate = (pre > 0) * factor if relu else factor.expand(rows, width)
+            check(out, pre * gate, factor * (8 * u * ((h * W).abs() + B.abs()) + h_off * W.abs()), dtype, ("out", *what))
+            g = grad.double() * gate
+            gw = g * W
+            c1, c2 = gw.mean(1, keepdim=True), (gw * h).mean(1, keepdim=True)
+            m1, m2 = gw.abs().mean(1, keepdim=True), (gw * h).abs().mean(1, keepdim=True)
+            want = rstd * (gw - c1 - h * c2)
+            off = rstd * (8 * u * (gw.abs() + m1 + h.abs() * m2) + (width / 64 + 16) * u * (m1 + h.abs() * m2) + 2 * h_off * m2
+                          + h_off.mean(1, keepdim=True) * m1 * h.abs()) + want.abs() * (width + 16) * 2.0 ** -52
+            check(dx, want, off, dtype, ("dx", *what))
+            chain = min(rows, 1024) + 64 + 4
+            check(dw, (g * h).sum(0), chain * u * (g * h).abs().sum(0) + (g.abs() * h_off).sum(0), params, ("dweight", *what))
+            check(db, g.sum(0), chain * u * g.abs().sum(0), params, ("dbias", *what))

@@ -13,6 +13,7 @@ from compressgnn_amd import build
 from CompressgnnDropout import Compressgnn_Dropout
 from CompressgnnNorm import Compressgnn_LayerNorm
 from launches import record
+from row_shapes import CODES, many
 
 
 # ------------------------------------------------------------------------- sources --
@@ -199,3 +200,28 @@ def test_no_sum_of_parts_is_built_that_no_call_takes(tmp_path):
     reached = {kernel for _, launches in results for kernel, _, _ in launches}
     built = {kernel for kernel in kernels if kernel[0] == "norm_sum_parts_kernel"}
     assert built <= reached, built - reached
+
+
+def test_every_kernel_of_the_norm_is_reached_by_the_tests_with_formulas(tmp_path):
+    """Each instance of the row kernels that the library has, type by type, ReLU and dropout in all four ways, is what one of the matrices
+    launches that are compared with the formulas in 64 bits on the GPU."""
+    from test_gpu_norm import SHAPES
+    calls, wanted = [], []
+    for dtype, code in CODES.items():
+        for param in {code, 0} if code > 1 else {code}:
+            for relu, kept in ((False, None), (True, None), (False, 45875), (True, 32768)):
+                for shape, (rows, width) in [(None, s) for s in SHAPES] + [(shape, (rows, width)) for shape, rows, width in many(dtype)]:
+                    for op in ("norm", "gradients"):
+                        calls.append(dict(op=op, rows=rows, F=width, dtype=code, param=param, relu=relu, kept=kept))
+                        wanted.append(shape if op == "norm" else None)
+    results, kernels = record(tmp_path, calls)
+    reached = set()
+    for call, shape, (status, launches) in zip(calls, wanted, results):
+        assert status == 0
+        reached.update(kernel for kernel, _, _ in launches)
+        if shape:
+            (name, values), = [kernel for kernel, _, _ in launches]
+            assert name == "norm_rows_kernel" and values[1:3] == shape, (call, name, values, shape)
+    missing = [kernel for kernel in kernels if kernel[0].startswith("norm_") and kernel not in reached]
+    assert not missing, sorted(missing)
+    assert sum(kernel[0] == "norm_rows_kernel" for kernel in reached) > 4 * 4 * 18
