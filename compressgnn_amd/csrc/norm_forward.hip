@@ -215,7 +215,7 @@ constexpr int64_t kLargeRounds = 8;
 
 template <typename T, bool RELU, bool DROP>
 int norm_launch(NormArgs<T> a, hipStream_t stream) {
-    const RowShape shape = row_shape(a.rows, a.F, sizeof(T), false);
+    const RowShape shape = row_shape(a.rows, a.F, sizeof(T), false, a.weight.wide);
     if (a.rows * a.F * (int64_t)sizeof(T) < 16) {
         hipLaunchKernelGGL((norm_few_kernel<T, RELU, DROP>), dim3(1), dim3(kWave), 0, stream, a);
         return check_launch("layer_norm");

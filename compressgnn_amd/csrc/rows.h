@@ -604,8 +604,11 @@ struct RowShape {
 // The same where the chip has lanes enough for about all packs at once, forward: there the time is that of one row's chain of loads
 // and additions, and a pack a lane makes it shortest (257 bfloat16 features: one row 3.0 against 5.5 us, 8,192 rows 8.3 against 9.6;
 // 1,000: one row 3.0 against 4.2, 4,096 rows 9.9 against 12.6).  16-bit rows of more than 256 packs, whose columns cost most, take it for
-// four times as many rows (float32 parameters: 2,400 float16 features, 1,500 rows 12 against 22 us, 3,000 18 against 23; 4,096 features,
-// 2,048 rows 17 against 21, 4,096 rows 23 against 25, with float16 ones 23 against 22; beyond the limit 8,192 rows 35 against 33).
+// more rows: under float32 parameters for four times as many (4,096 features: 2,048
+// rows 15.6 against 20.4 us, 4,096 rows 21.1 against 23.8; 2,400: 4,096 rows 19.1 against 24.2; at 8,192 rows of 4,096 it loses, 35 against 33);
+// under their own for three and a half times (4,096 features: 2,048 rows 12.8 against 14.2, 3,500 rows 16.6 against 17.0; 2,400: 3,500 rows 15.5
+// against 17.2; at 4,096 rows it loses, among others 19.5 against 19.0, alone 22.0 against 19.9, where ReLU and dropout are behind it 24.2 and
+// 24.8, from memory alone 22.4 and 23.7; 6,000 rows 23.4 against 22.4).
 constexpr int64_t kAtOnce = 1 << 19;
 
 inline RowShape spread_shape(int64_t packs) {
@@ -613,10 +616,10 @@ inline RowShape spread_shape(int64_t packs) {
     return {pow2_ceil(packs), 1, std::max(pow2_ceil(packs), packs > kWave ? 128 : kBlock)};
 }
 
-inline RowShape row_shape(int64_t rows, int64_t F, size_t element, bool gradient) {
+inline RowShape row_shape(int64_t rows, int64_t F, size_t element, bool gradient, bool wide = false) {
     const int64_t packs = ceil_div(F, 16 / (int64_t)element);
     const RowShape spread = spread_shape(packs);
-    const int64_t at_once = element == 2 && packs > 256 ? 4 * kAtOnce : kAtOnce;
+    const int64_t at_once = element == 2 && packs > 256 ? (wide ? 8 : 7) * kAtOnce / 2 : kAtOnce;
     if (!gradient && spread.lanes && rows * spread.lanes <= at_once) return spread;
     if (packs > (gradient && element == 2 ? 1024 : 2048)) return {0, 0, 0};
     if (packs <= 3) return {1, (int)packs, kBlock};

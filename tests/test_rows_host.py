@@ -225,3 +225,12 @@ def test_every_kernel_of_the_norm_is_reached_by_the_tests_with_formulas(tmp_path
     missing = [kernel for kernel in kernels if kernel[0].startswith("norm_") and kernel not in reached]
     assert not missing, sorted(missing)
     assert sum(kernel[0] == "norm_rows_kernel" for kernel in reached) > 4 * 4 * 18
+
+
+@pytest.mark.parametrize("dtype", [2, 3])
+@pytest.mark.parametrize("rows,param,packs", [(2048, 0, 1), (4096, 0, 1), (4097, 0, 2), (2048, 2, 1), (3584, 2, 1), (3585, 2, 2), (4096, 2, 2)])
+def test_wide_16_bit_rows_are_spread_where_that_was_faster(tmp_path, dtype, rows, param, packs):
+    """4,096 features: a pack a lane under float32 parameters up to 4,096 rows, under parameters of the rows' type only where it gained."""
+    (_, launches), = record(tmp_path, [dict(op="norm", rows=rows, F=4096, dtype=dtype, param=dtype if param == 2 else 0)])[0]
+    (name, values), = [kernel for kernel, _, _ in launches]
+    assert name == "norm_rows_kernel" and values[1:3] == ((512, 1) if packs == 1 else (256, 2))
