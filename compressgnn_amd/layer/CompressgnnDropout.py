@@ -43,7 +43,7 @@ def dropout(x, p, seed, offset=0, counter=None):
 
 def _fresh_seed():
     """Of torch's own generator, where none is given: torch.manual_seed fixes it, and no two modules share masks."""
-    return int(torch.randint(1 << 62, (1,)))
+    return int(torch.randint(1 << 62, (1,), device="cpu"))  # whatever device modules are being made on, the one without memory too
 
 
 _numbering = threading.Lock()  # no two calls get one number, whatever threads they come from

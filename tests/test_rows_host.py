@@ -141,6 +141,20 @@ def test_deep_copies_draw_masks_of_their_own():
     assert (same[1].seed, same[1].calls, same[2].seed) == (before, 7, layer[2].seed)
 
 
+def test_modules_are_made_on_the_device_without_memory():
+    """As large models are laid out before their weights are there."""
+    with torch.device("meta"):
+        layers = torch.nn.Sequential(Compressgnn_LayerNorm(4, p=0.5), Compressgnn_Dropout(0.5))
+        stack = [copy.deepcopy(layers) for _ in range(2)]
+    assert layers[0].weight.is_meta and layers[1].replays.is_meta
+    assert len({module.seed for layers in [layers, *stack] for module in layers}) == 6
+    torch.manual_seed(3)
+    seed = Compressgnn_Dropout(0.5).seed
+    torch.manual_seed(3)
+    with torch.device("meta"):
+        assert Compressgnn_Dropout(0.5).seed == seed
+
+
 def test_calls_from_two_threads_get_two_numbers():
     """A second call that comes while the first is between reading the count and writing it: forced, not hoped for."""
     numbers = {}
