@@ -42,8 +42,8 @@ __device__ __forceinline__ void leave_sum(compute_t<T> *part, void *whole, bool 
 
 // Rows that fit the registers of their lanes, as in the forward pass: x and the gradient are read once for dx and for
 // the parameters' sums, which every lane holds for its own columns until its rows are through.  Bound as the forward pass is:
-// 2,449,029 rows of 256 float32 features with ReLU and dropout 1,434 us, 5.2 of the 6.0 TB/s that two matrices in and one out reach;
-// 325,557 of 257 float16 features 140 us, ALU 77 % busy.
+// 2,449,029 rows of 256 float32 features with ReLU and dropout 1,438 us, 5.2 of the 6.0 TB/s that two matrices in and one out reach;
+// 325,557 of 257 float16 features 147 us, ALU 75 % busy.
 template <typename T, int LANES, int K, int THREADS, bool RELU, bool DROP>
 __global__ __launch_bounds__(THREADS) void norm_gradients_kernel(NormArgs<T> a) {
     using C = compute_t<T>;

@@ -10,9 +10,9 @@ namespace {
 
 // Rows that fit the registers of their lanes: LANES of them hold K packs of 16 bytes each, so a row is read once and
 // written once.  The packs of the next row are asked for before this one's are used.  Bound by memory for whole packs of
-// four-byte elements (2,449,029 rows of 256 float32 features with ReLU and dropout: 886 us, 5.7 TB/s of the 6.2 that a copy
-// reaches), by the vector ALU for 16-bit rows of odd widths (325,557 of 257 float16 features, the same: 116 us, 2.9 TB/s, ALU
-// 76 % busy: conversions, sums in 64 bits and the generator cost an element of two bytes what they cost one of four).
+// four-byte elements (2,449,029 rows of 256 float32 features with ReLU and dropout: 905 us, 5.5 TB/s of the 6.2 that a copy
+// reaches), by the vector ALU for 16-bit rows of odd widths (325,557 of 257 float16 features, the same: 125 us, 2.7 TB/s, ALU
+// 72 % busy: conversions, sums in 64 bits and the generator cost an element of two bytes what they cost one of four).
 template <typename T, int LANES, int K, int THREADS, bool RELU, bool DROP>
 __global__ __launch_bounds__(THREADS) void norm_rows_kernel(NormArgs<T> a) {
     using C = compute_t<T>;
@@ -100,8 +100,8 @@ __global__ __launch_bounds__(THREADS) void norm_rows_kernel(NormArgs<T> a) {
     }
 }
 
-// Longer rows: a workgroup a row, which reads it twice (float64: three times), kLongPacks packs a lane at a time.  Bound by the latency of the two
-// readings, one workgroup a compute unit (3,000 rows of 20,000 float32 features: 208 us, 2.3 TB/s; a pack at a time 299).
+// Longer rows: a workgroup a row, which reads it twice (float64: three times), kLongPacks packs a lane at a time.  Bound by the latency of the
+// readings, one workgroup a compute unit (3,000 rows of 20,000 float32 features: 206 us, 2.3 TB/s; a pack at a time 299; float64 278 us, 3.5 TB/s).
 template <typename T, bool RELU, bool DROP>
 __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(NormArgs<T> a) {
     using C = compute_t<T>;
@@ -226,7 +226,8 @@ int norm_launch(NormArgs<T> a, hipStream_t stream) {
     }
     // Over and over the chip's width, or, from a gigabyte on, a few rounds of neighbouring rows for each of more workgroups, so that none gets
     // far ahead of the others (2,449,029 rows of 256 features with ReLU and dropout, float32: 909 us, 1,026 the other way, bfloat16:
-    // 492 and 548; 300,000 of 602, bfloat16: 171 and 150).
+    // 492 and 548; 300,000 of 602, bfloat16: 171 and 150).  Below the limit (float32, no ReLU, no dropout) the width tells more than the bytes: 100, 128
+    // and 256 features cross at 0.7 GB (0.5 GB: 2 % lost, 0.95 GB: 1 to 2 % gained), 47 lose 9 % from 0.5 to 0.95 GB, 300 and 602 gain 9 to 15 % there.
     const int64_t bytes = a.rows * a.F * (int64_t)sizeof(T), groups = shape.threads / shape.lanes, tiles = ceil_div(a.rows, groups);
     int64_t workgroups = row_workgroups(a.rows, shape, sizeof(T), false);
     a.walk = {groups, groups * workgroups, ceil_div(tiles, workgroups)};

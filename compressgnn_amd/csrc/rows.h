@@ -561,8 +561,10 @@ struct Centre {
 
 // h = (x - m) r and v = h w + b of a pack.  Forward pass and gradient call this with the same numbers, and with RELU the
 // side of zero that v is on is that of its value in 64 bits: h takes three roundings and v one more, so v is less than
-// 2^-22 (|b| + |v|) off and its sign is certain where |v| > 2^-21 |b|; the few packs that come closer (one of 100,000) are
-// computed again.  A float decision alone would let a sum over a million elements be a whole gradient off now and then.
+// 2^-22 (|b| + |v|) off and its sign is certain where |v| > 2^-21 |b|; packs that come closer are computed again: one of
+// 100,000 of those that the row fills, and in every row those that reach behind its end, where weight, bias and so v are zero (257
+// features in places for 384: the third pack of each lane).  A float decision alone would let a sum over a million elements be a whole
+// gradient off now and then.
 template <bool RELU, int N, typename T, typename C>
 __device__ __forceinline__ void normalised(const Pack<T, N> &x, const Centre<C> &centre, const C (&w)[N], const C (&b)[N], C (&h)[N], C (&v)[N]) {
 #pragma unroll

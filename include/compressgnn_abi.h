@@ -450,7 +450,8 @@ int cgnn_dropout(int64_t rows, int64_t F, int dtype, const void *x, int64_t ldx,
 /* out = drop(relu((x - m) r w + b)), m and v the mean of a row and of its squares around it, r = 1 / sqrt(v + eps);
  * weight, bias (NULL: 1, 0) of type param_dtype, which is dtype or, for 16-bit rows, CGNN_F32; relu 0: without;
  * drop NULL: nothing dropped.  stats: [rows, 2], m and r of every row for the gradient, or NULL.  m, v, r and the
- * value that the ReLU looks at are computed in 64 bits. */
+ * value that the ReLU looks at are computed in 64 bits; of float and 16-bit rows x - m and r have to be finite as floats, of float64
+ * rows the squares of x - m. */
 int cgnn_layer_norm(int64_t rows, int64_t F, int dtype, int param_dtype, const void *x, int64_t ldx, const void *weight,
                     const void *bias, double eps, int relu, const cgnn_drop *drop, void *out, double *stats,
                     cgnn_stream_t stream);
