@@ -103,7 +103,7 @@ class Masks:
         missing = []
         super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing, unexpected_keys, error_msgs)
         place = {prefix + "replays", prefix + "_extra_state"}
-        missing_keys += [key for key in missing if key not in place or not place.isdisjoint(state_dict)]
+        missing_keys += [key for key in missing if key not in place or any(part in state_dict for part in place)]
 
 
 class Compressgnn_Dropout(Masks, torch.nn.Module):
